@@ -1,0 +1,38 @@
+// 8-bit floating point (e4m3: 4 bits of exponent, 3 of mantissa, largest value 448) with a scale for each block of 128.
+//
+// A block x of 128 values (of a row, or of 128 x 128 of a matrix) is held as
+//   m = max(max |x|, 2^-100)   (NaN where an x is),   scale = m / 448,   q = e4m3(x * (448 / m)),
+// every step one operation in 32 bits, rounded to nearest.  The floor keeps 448 / m finite; a block of zeros is zeros.  A block with an
+// infinity has an infinite scale and NaN in that place, one with a NaN is NaN throughout: both make the outputs that they enter NaN.
+#pragma once
+#include "common.cuh"
+
+constexpr int F8_BLOCK = 128;
+
+__device__ __forceinline__ float max_nan(float a, float b) {           // NaN where either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+struct BlockScale { float scale, inverse; };
+__device__ __forceinline__ BlockScale block_scale(float most) {
+  const float m = max_nan(most, 0x1p-100f);
+  return {__fdiv_rn(m, 448.f), __fdiv_rn(448.f, m)};
+}
+// four values as e4m3, the first in the lowest byte
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;\n" : "=h"(lo) : "f"(a), "f"(b));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;\n" : "=h"(hi) : "f"(c), "f"(d));
+  return (uint32_t)hi << 16 | lo;
+}
+
+// D (16x8, f32) += A (16x32, e4m3, row) * B (32x8, e4m3, col); with g = lane / 4, c = lane % 4 and four values a register
+//   a0 = A[g][4c..]  a1 = A[g+8][4c..]  a2 = A[g][4c+16..]  a3 = A[g+8][4c+16..]   b0 = B[4c..][g]  b1 = B[4c+16..][g]
+//   d0,d1 = D[g][2c,2c+1]  d2,d3 = D[g+8][2c,2c+1]
+__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}

@@ -22,7 +22,8 @@ __all__ = ["KernelError", "KernelBuildError", "embed_rows", "rmsnorm", "qknorm_r
            "canon_conv", "norm_canon_single", "latent_keep", "head_product", "head_gate", "gated_add", "xielu",
            "proj_norm_rope_cache", "rotate_heads", "short_conv", "state_scan", "head_norm_gate", "gate_mul",
            "norm_add", "norm_shift", "scan_gates_step", "scan_gates_max", "state_readout", "pool_update", "moe_route", "moe_plan", "moe_gemm", "moe_gemv", "moe_gather", "moe_gemm_tc", "moe_combine", "moe_combine_norm_add", "moe_tile_rows", "tanh_norm", "scaled_join", "relu2", "selective_scan", "diff_combine", "GluForm", "norm_join", "moe_combine_join", "latent_pair",
-           "channel_scan", "stream_add", "embed_norm_rows", "streams_read", "streams_join", "shift_mix", "latent_rope", "act_form", "linear_act", "linear_stacked", "head_expand_tiles"]
+           "channel_scan", "stream_add", "embed_norm_rows", "streams_read", "streams_join", "shift_mix", "latent_rope", "act_form", "linear_act", "linear_stacked", "head_expand_tiles",
+           "Fp8Rows", "Fp8Matrix", "Fp8Matrices", "quantize_rows", "quantize_matrix", "moe_sort", "moe_experts_fp8", "moe_back"]
 
 F32, BF16 = 0, 1
 EPI_STORE_F32, EPI_STORE_BF16, EPI_ACCUM_F32 = 0, 1, 2
@@ -84,6 +85,7 @@ def _need(t: torch.Tensor, dtype: torch.dtype, what: str) -> None:
 
 _fn_cache: dict = {}
 _bf16 = None              # the bfloat16 bindings (they import this module, so they are bound at first use)
+_fp8 = None               # and those of 8-bit floating point
 
 
 def _bf16_mod():
@@ -92,6 +94,14 @@ def _bf16_mod():
         from . import kernels_bf16 as m
         _bf16 = m
     return _bf16
+
+
+def _fp8_mod():
+    global _fp8
+    if _fp8 is None:
+        from . import kernels_fp8 as m
+        _fp8 = m
+    return _fp8
 
 
 def _fn(unit: str, name: str, argtypes, defines=()):
@@ -166,6 +176,43 @@ class GluForm(NamedTuple):
 
 SILU = GluForm()
 _GLU_TYPES = [c_float, c_float, c_float, c_float]
+
+
+class Fp8Rows(NamedTuple):
+    """Rows of activations in 8-bit floating point (csrc/fp8.cuh): ``q`` float8_e4m3fn [T, K filled up with zeros to whole blocks of 128], ``scale``
+    float32 [blocks, T]; the value k of row t is q[t, k] * scale[k // 128, t]."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+class Fp8Matrix(NamedTuple):
+    """A matrix [N, ``k``] in 8-bit floating point with a scale for every 128 x 128: ``q`` float8_e4m3fn [N, k filled up with zeros to whole
+    blocks], ``scale`` float32 [ceil(N / 128), ceil(k / 128)].  A gate/up matrix has rows alternating in eights and scales [2, ceil(N / 256), ..], the
+    gate's and the up's; a stack of matrices has one more axis in front of both."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    @property
+    def shape(self):
+        return torch.Size((*self.q.shape[:-1], self.k))
+
+    @property
+    def dtype(self):
+        return self.q.dtype
+
+
+class Fp8Matrices(NamedTuple):
+    """Matrices in 8 bits whose outputs lie side by side although their rows do not fill blocks of 128."""
+    parts: tuple
+
+    @property
+    def shape(self):
+        return torch.Size((sum(m.q.shape[0] for m in self.parts), self.parts[0].k))
+
+    @property
+    def dtype(self):
+        return self.parts[0].dtype
 
 
 def embed_rows(table: torch.Tensor, ids: torch.Tensor, out: torch.Tensor, scale: float = 1.0, positions=None,
@@ -694,7 +741,10 @@ def gemm_f32_tc(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, accumulate:
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, accumulate: bool = False, workspace=None) -> None:
     """The product a layer asks for; picks the kernel from the dtypes and sizes.  Anything
     that is not all-bfloat16 runs on the float32 kernel (true 32-bit arithmetic), but for many rows in float32 with a
-    ``workspace`` for their parts (``gemm_f32_tc``)."""
+    ``workspace`` for their parts (``gemm_f32_tc``).  With ``w`` in 8 bits (``Fp8Matrix``, ``Fp8Matrices``) ``a`` is quantised first (in the
+    workspace, or in new memory without one) unless it is ``Fp8Rows``; out is float32 or bfloat16."""
+    if isinstance(w, (Fp8Matrix, Fp8Matrices)):
+        return (_fp8 or _fp8_mod()).linear(a, w, out, accumulate, workspace)
     if a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16:
         if (_bf16 or _bf16_mod()).linear_bf16(a, w, out, accumulate):
             return
@@ -725,11 +775,22 @@ def linear_act(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, form: GluFor
     return False
 
 
+def quantize_rows(x: torch.Tensor, rows: Fp8Rows, pair_row: Optional[torch.Tensor] = None) -> None:
+    """``rows`` = x [T, K] (float32 or bfloat16) in 8 bits, a scale for every row and 128 columns.  ``pair_row`` int32 [T, top]: row t
+    goes to the rows ``pair_row[t]`` instead, to none for those below zero (what ``moe_sort`` leaves)."""
+    (_fp8 or _fp8_mod()).quantize_rows(x, rows, pair_row)
+
+
+def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
+    """A matrix [N, K], or a stack [E, N, K], of float32 or bfloat16 in 8 bits, a scale for every 128 x 128."""
+    return (_fp8 or _fp8_mod()).quantize_matrix(w)
+
+
 def product_notices(what: str, w: Optional[torch.Tensor], compute_dtype: torch.dtype) -> list:
     """Why products with the matrix ``w`` will run on the 32-bit FFMA kernel although the
     model computes in bfloat16: one line per reason, for the notice printed when a model is
     built (the result is right either way; the speed is not the same)."""
-    if w is None or compute_dtype != torch.bfloat16:
+    if w is None or compute_dtype != torch.bfloat16 or isinstance(w, (Fp8Matrix, Fp8Matrices)):
         return []
     if w.dtype != torch.bfloat16:
         return [f"{what}: the matrix is kept in {str(w.dtype).replace('torch.', '')} as stored, so its "
@@ -910,9 +971,15 @@ def normed_product(x32, eps, w, out, gate_block=None) -> bool:
     return False
 
 
-def gate_up_fused(h, w_gate_up, mid, block, form: GluForm = SILU) -> bool:
+def gate_up_fused(h, w_gate_up, mid, block, form: GluForm = SILU, workspace=None) -> bool:
     """silu(gate) * up (or another gate of ``GluForm``'s kind) computed inside the product's epilogue; False when
-    no kernel takes the case (the caller then runs the product and ``swiglu`` separately)."""
+    no kernel takes the case (the caller then runs the product and ``swiglu`` separately).  A gate/up matrix in 8 bits (rows in eights)
+    takes ``h`` as ``linear`` does and leaves ``mid`` in float32 or, given ``Fp8Rows``, as the rows of the product that follows."""
+    if isinstance(w_gate_up, Fp8Matrix):
+        if block != 8:
+            raise KernelError(f"gate_up_fused: a gate/up matrix in 8 bits alternates in eights, not {block}")
+        (_fp8 or _fp8_mod()).gate_up(h, w_gate_up, mid, form, workspace)
+        return True
     if h.dtype == torch.bfloat16 and w_gate_up.dtype == torch.bfloat16:
         return (_bf16 or _bf16_mod()).gate_up_bf16(h, w_gate_up, mid, block, form)
     return False
@@ -1483,6 +1550,25 @@ def moe_combine(rows32, pair_row, weight, x_self32, top: int, out32, accumulate:
                                           c_void_p])
     _call(f, _ptr(rows32), _ptr(pair_row), _ptr(weight), _ptr(x_self32), out32.shape[0], top, out32.shape[1],
           _ptr(out32), 1 if accumulate else 0, _stream())
+
+
+def moe_sort(idx, n_real: int, starts, pair_row) -> None:
+    """Rows for the (token, choice) pairs of ``idx`` int32 [T, top], expert by expert and, within an expert, in the pairs' order: ``starts``
+    int32 [n_real + 1], ``pair_row`` int32 like ``idx`` (-1: an expert from ``n_real`` on, which has no matrices)."""
+    (_fp8 or _fp8_mod()).moe_sort(idx, n_real, starts, pair_row)
+
+
+def moe_experts_fp8(h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, pair_row, form: GluForm = SILU, workspace=None) -> None:
+    """The experts' part of a routed feed-forward with matrices in 8 bits: the tokens ``h`` [T, K] quantised and sorted by the experts ``idx``
+    int32 [T, top] (``moe_sort``), each expert's gated product over its rows, quantised again, and its down product: ``rows32`` float32
+    [T * top, H] (rows without a pair stay as they are) and ``pair_row``, for ``moe_back`` and the other combinations."""
+    (_fp8 or _fp8_mod()).moe_experts(h, idx, w_gate_up, w_down, rows32, pair_row, form, workspace)
+
+
+def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool = False) -> None:
+    """out[t] = sum_j weight[t, j] * (rows32[pair_row[t, j]], or x_self[t] where the pair has no row), the choices in their order; ``x_self`` float32 or
+    bfloat16, ``out`` float32 (``accumulate``: added to) or bfloat16."""
+    (_fp8 or _fp8_mod()).moe_back(rows32, pair_row, weight, x_self, out, accumulate)
 
 
 def moe_combine_norm_add(rows32, pair_row, weight, x32, norm_w, eps: float, top: int, cast_out=None) -> bool:
