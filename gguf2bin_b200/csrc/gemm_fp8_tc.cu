@@ -1,0 +1,419 @@
+// Products in 8-bit floating point (fp8.cuh) of many rows, on the 5th-generation tensor cores:
+//   C[t, n] = sum_b s[b, t] S[n / 128, b] sum_{k in block b} q[t, k] Q[n, k].
+//
+// The scales change every 128 of K, so no accumulator can run over all of K: a block's sums are formed in tensor memory (four
+// tcgen05.mma of kind::f8f6f4, M = N = 256, K = 32, a pair of CTAs) and added, times the two scales, to sums in registers.
+// Roles by warp, a pair of CTAs a tile of 256 x 256 (each its own 128 rows), one pair after another of the persistent grid:
+//   warp 8   copies: a block of K of the CTA's rows of A and of its half of W's 256 (128-byte swizzle), STAGES in flight
+//   warp 9   products, in the pair's first CTA, into one of two accumulators of 256 columns
+//   warps 0-7  add: warp w reads lanes 32 (w % 4) .. + 31 (a thread owns a row of A, so its scale is one number a block) and columns
+//              128 (w / 4) .. + 127 (one block of W's rows: one number too) of a finished accumulator while the other one is filled;
+//              behind the last block they write C, through shared memory, in rows
+//
+// `starts`: W is a stack of matrices and rows starts[e] .. starts[e + 1] of A meet the e-th.  Gated: rows of W alternate, eight gates and the eight
+// ups of the same outputs, each with the scales of their own matrix; a tile is then 128 outputs wide, one block of the rows that the next product
+// reads, so their scale is known where they are made.
+//
+// Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
+#include "fp8.cuh"
+#include "glu.cuh"
+#include "tc_common.cuh"
+
+G2B_DEFINE_LAST_ERROR
+
+using namespace tc;
+
+enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3, EPI_GATED_ROWS = 4 };
+enum { ST_PRODUCER_TIMEOUT = 31, ST_MMA_TIMEOUT = 32, ST_ADDER_TIMEOUT = 33 };
+
+constexpr int BM = 128, BN = 256, BK = F8_BLOCK;        // BM: rows of a CTA
+constexpr int PART_BYTES = BM * BK, STAGE_BYTES = 2 * PART_BYTES;
+constexpr int STAGES = 5;
+constexpr int ADDERS = 8, THREADS = (ADDERS + 4) * 32;   // the last two warps only complete a group of four
+// Registers: 384 threads start with 168 each (64,512); the adders hold 128 sums and two pieces of an accumulator and take 232, the others
+// keep 40: 256 * 232 + 128 * 40 = 64,512.
+constexpr int ADDER_REGS = 232, OTHER_REGS = 40;
+constexpr int COLS = BN / 2, AT_ONCE = 16;
+constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+constexpr int PITCH = 36;                                // floats a row of an adder's 32 x 32 outputs on their way to C
+constexpr int OUT_BYTES = ADDERS * 32 * PITCH * 4;
+constexpr int MOST_EXPERTS = 1024;
+constexpr int BAR_BYTES = 256, LIST_BYTES = (MOST_EXPERTS + 1) * 4;
+constexpr int SMEM = RING_BYTES + OUT_BYTES + 1024 + BAR_BYTES;                        // + the swizzle's alignment
+constexpr int SMEM_GROUPED = SMEM + LIST_BYTES;
+static_assert(SMEM_GROUPED <= 227 * 1024, "one CTA a multiprocessor");
+constexpr int BAND = 8;                                  // tiles along M that are walked side by side
+
+struct Tc {
+  const float *sa, *sw;
+  void *out;
+  float *out_scale;                                      // EPI_GATED_ROWS: [blocks of the outputs, ldos]
+  const int *starts;
+  int *status;
+  int M, N, blocks, n_experts, nb;                       // nb: blocks of W's rows that have a scale
+  long long lds, ldo, ldos;
+  GluForm form;
+};
+
+template <bool ACC>
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  constexpr uint32_t HIGH = (1024 >> 4) | (1u << 14) | (2u << 29);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}\n"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(HIGH), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+// Waits for this thread's loads of tensor memory; the registers pass through, so that nothing that reads them moves in front.
+__device__ __forceinline__ void loaded16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+// One arrival on a barrier of the pair: this warp's reads of tensor memory are done (they are waited for); it hands over no data.
+__device__ __forceinline__ void arrive_read(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_bar) : "memory");
+}
+// accumulator float, both operands e4m3 and K-major
+constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(2 * BM >> 4) << 24);
+
+struct Tile { int e, m0, end, n0; };
+
+// Tile t of the walk.  `list`: with experts, list[e] = tiles of the experts up to e along M (in shared memory).
+template <bool GROUPED>
+__device__ __forceinline__ Tile find_tile(const Tc &p, const int *list, int t, int tiles_n) {
+  Tile r;
+  if (GROUPED) {
+    int lo = 0, hi = p.n_experts - 1;                    // the first expert with list[e] * tiles_n > t
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (list[mid] * tiles_n > t) hi = mid;
+      else lo = mid + 1;
+    }
+    const int before = lo ? list[lo - 1] : 0, high = list[lo] - before, at = t - before * tiles_n;
+    r.e = lo, r.n0 = at / high * BN, r.m0 = p.starts[lo] + at % high * 2 * BM, r.end = p.starts[lo + 1];
+  } else {
+    const int tiles_m = (p.M + 2 * BM - 1) / (2 * BM), band = t / (BAND * tiles_n), high = min(BAND, tiles_m - band * BAND), at = t - band * BAND * tiles_n;
+    r.e = 0, r.n0 = at / high * BN, r.m0 = (band * BAND + at % high) * 2 * BM, r.end = p.M;
+  }
+  return r;
+}
+
+template <int EPI, bool GROUPED>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Tc p) {
+  constexpr bool GATED = EPI == EPI_GATED_F32 || EPI == EPI_GATED_ROWS;
+  pdl_launch();
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + RING_BYTES + OUT_BYTES);
+  const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * STAGES, sum_full0 = empty0 + 8 * STAGES, sum_empty0 = sum_full0 + 16;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 4);
+  int *list = reinterpret_cast<int *>(smem + RING_BYTES + OUT_BYTES + BAR_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t half = cluster_ctarank();               // the pair's first CTA issues its products
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);                       // in the first CTA, with both CTAs' bytes
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(sum_full0 + 8 * b, 1);
+      mbar_init(sum_empty0 + 8 * b, 2 * ADDERS);         // in the first CTA: both CTAs' adders
+    }
+    mbar_init_fence();
+  }
+  if (warp == ADDERS + 1) tmem_alloc_pair(smem_addr(tmem_slot), 2 * BN);
+  pdl_wait();
+  const int tiles_n = (p.N + BN - 1) / BN;
+  int n_tiles;
+  if (GROUPED) {
+    if (warp == 0) {                                     // tiles of the experts, summed up 32 at a time
+      int sum = 0;
+      for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
+        const int e = e0 + lane;
+        int v = e < p.n_experts ? (p.starts[e + 1] - p.starts[e] + 2 * BM - 1) / (2 * BM) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, v, o);
+          if (lane >= o) v += u;
+        }
+        if (e < p.n_experts) list[e] = sum + v;
+        sum += __shfl_sync(0xffffffffu, v, 31);
+      }
+    }
+  }
+  tc_fence_before();
+  cluster_sync_all();                                    // both CTAs' barriers, tensor memory and lists exist
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (GROUPED) n_tiles = list[p.n_experts - 1] * tiles_n;
+  else n_tiles = (p.M + 2 * BM - 1) / (2 * BM) * tiles_n;
+  const int pairs = gridDim.x / 2, pair = blockIdx.x / 2;
+
+  if (warp >= ADDERS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
+    if (warp == ADDERS && lane == 0 && PRODUCER_RUNS) {
+      const uint32_t first_full0 = map_to_cta(full0, 0);
+      bool ok = true;
+      int it = 0;
+      for (int t = pair; t < n_tiles && ok; t += pairs) {
+        const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
+        const int row_a = tile.m0 + (int)half * BM, row_w = tile.e * p.N + tile.n0 + (int)half * BM;
+        for (int b = 0; b < p.blocks; ++b, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !mbar_wait(empty0 + 8 * s, (it / STAGES - 1) & 1)) {
+            atomicExch(p.status, ST_PRODUCER_TIMEOUT);
+            ok = false;
+            break;
+          }
+          const uint32_t to = smem_addr(smem + s * STAGE_BYTES);
+          if (half == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+          tma_load_2d_pair(to, &map_a, b * BK, row_a, first_full0 + 8 * s);
+          tma_load_2d_pair(to + PART_BYTES, &map_w, b * BK, row_w, first_full0 + 8 * s);
+        }
+      }
+    }
+    if (warp == ADDERS + 1 && lane == 0 && half == 0) {
+      bool ok = true;
+      int it = 0;
+      for (int t = pair; t < n_tiles && ok; t += pairs)
+        for (int b = 0; b < p.blocks; ++b, ++it) {
+          const int s = it % STAGES, h = it & 1;
+          if ((it >= 2 && !mbar_wait_cluster(sum_empty0 + 8 * h, (it / 2 - 1) & 1)) || !mbar_wait(full0 + 8 * s, (it / STAGES) & 1)) {
+            atomicExch(p.status, ST_MMA_TIMEOUT);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t lo = ((smem_addr(smem + s * STAGE_BYTES) & 0x3FFFF) >> 4) | 1u << 16;
+          const uint32_t to = tmem + h * BN;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (k == 0) umma_f8_pair<false>(to, lo, lo + PART_BYTES / 16, IDESC);
+            else umma_f8_pair<true>(to, lo + 2 * k, lo + PART_BYTES / 16 + 2 * k, IDESC);
+          }
+          umma_commit_pair(empty0 + 8 * s, 3);
+          umma_commit_pair(sum_full0 + 8 * h, 3);
+        }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(ADDER_REGS));
+    const int row0 = 32 * (warp % 4), col0 = COLS * (warp / 4);
+    const uint32_t first_empty0 = map_to_cta(sum_empty0, 0);
+    const uint32_t from0 = tmem + ((uint32_t)row0 << 16) + col0;
+    float *const mid = reinterpret_cast<float *>(smem + RING_BYTES) + warp * 32 * PITCH;
+    bool ok = true;                                      // once a wait gave up nothing is waited for any more, and (but with EPI_GATED_ROWS, whose warps
+    int it = 0;                                          // meet in pairs at every tile) nothing is written
+    for (int t = pair; t < n_tiles; t += pairs) {
+      const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
+      const int m0 = tile.m0 + (int)half * BM + row0, row = m0 + lane;
+      const float *sa = p.sa + min(row, p.M - 1);
+      // the scales of the thread's columns: one block of W's rows; gated, one of the gate's and one of the up's
+      const int n_block = GATED ? tile.n0 / 2 / F8_BLOCK : min((tile.n0 + col0) / F8_BLOCK, p.nb - 1);
+      const float *sw = p.sw + ((long long)tile.e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks;
+      const float *sw_up = sw + (long long)p.nb * p.blocks;
+      float sum[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
+      float next_a = sa[0], next_w = sw[0], next_up = GATED ? sw_up[0] : 0.f;
+      for (int b = 0; b < p.blocks; ++b, ++it) {
+        const int h = it & 1;
+        const float f = next_a * next_w, f_up = next_a * next_up;
+        if (b + 1 < p.blocks) {
+          next_a = sa[(b + 1) * p.lds];
+          next_w = sw[b + 1];
+          if (GATED) next_up = sw_up[b + 1];
+        }
+        if (!ok) continue;
+        ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (it / 2) & 1));      // the warp's lanes agree: its loads are all lanes'
+        if (!ok) {
+          if (lane == 0) atomicExch(p.status, ST_ADDER_TIMEOUT);
+          continue;
+        }
+        tc_fence_after();
+        uint32_t x[2][AT_ONCE];
+        tmem_ld16(from0 + h * BN, x[0]);
+#pragma unroll
+        for (int c = 0; c < COLS; c += AT_ONCE) {
+          const int cur = c / AT_ONCE & 1;
+          loaded16(x[cur]);
+          if (c + AT_ONCE < COLS) tmem_ld16(from0 + h * BN + c + AT_ONCE, x[cur ^ 1]);
+#pragma unroll
+          for (int j = 0; j < AT_ONCE; j += 2) {
+            const float fj = GATED && (j & 8) ? f_up : f;
+            const float2 v = fma2(make_float2(__uint_as_float(x[cur][j]), __uint_as_float(x[cur][j + 1])), make_float2(fj, fj),
+                                  make_float2(sum[c + j], sum[c + j + 1]));
+            sum[c + j] = v.x, sum[c + j + 1] = v.y;
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_read(first_empty0 + 8 * h);
+      }
+      if (!ok && EPI != EPI_GATED_ROWS) break;
+      const int rows = min(32, tile.end - m0);           // of this warp's that exist (may be none)
+      if (GATED) {
+        const int n_out = p.N / 2, out0 = (tile.n0 + col0) / 2;                        // 64 outputs a thread
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < COLS / 2; ++j) {
+          const int c = (j >> 3) * 16 + (j & 7);
+          float v = glu_value_fast(sum[c], sum[c + 8], p.form);
+          if (out0 + j >= n_out) v = 0.f;
+          sum[j] = v;
+          most = max_nan(most, fabsf(v));
+        }
+        if (EPI == EPI_GATED_ROWS) {
+          float *const given = mid;                      // the largest of a row: of the two warps that share it
+          given[lane] = most;
+          asm volatile("bar.sync %0, 64;\n" ::"r"(1 + warp % 4) : "memory");
+          most = max_nan(most, (mid + (warp < 4 ? 4 : -4) * 32 * PITCH)[lane]);
+          const BlockScale s = block_scale(most);
+          if (lane < rows) {
+            if (warp < 4) p.out_scale[tile.n0 / 2 / F8_BLOCK * p.ldos + row] = s.scale;
+            uint8_t *to = static_cast<uint8_t *>(p.out) + row * p.ldo + out0;
+#pragma unroll
+            for (int j = 0; j < COLS / 2; j += 16) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                w[i] = pack_e4m3(sum[j + 4 * i] * s.inverse, sum[j + 4 * i + 1] * s.inverse, sum[j + 4 * i + 2] * s.inverse, sum[j + 4 * i + 3] * s.inverse);
+              *reinterpret_cast<uint4 *>(to + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          asm volatile("bar.sync %0, 64;\n" ::"r"(1 + warp % 4) : "memory");     // the next tile's largest go where this one's were
+          continue;
+        }
+      }
+      if (rows <= 0) continue;
+      // 32 x 32 outputs at a time through shared memory, eight lanes a row
+      constexpr int OUTS = GATED ? COLS / 2 : COLS;
+      const int n_out = GATED ? p.N / 2 : p.N, first = GATED ? (tile.n0 + col0) / 2 : tile.n0 + col0;
+      const int c = 4 * (lane % 8);
+      const bool vector = p.ldo % 4 == 0 && ((uintptr_t)p.out & (EPI == EPI_BF16 ? 7 : 15)) == 0;
+#pragma unroll
+      for (int q = 0; q < OUTS / 32; ++q) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4 *>(mid + lane * PITCH + 4 * j) =
+              make_float4(sum[32 * q + 4 * j], sum[32 * q + 4 * j + 1], sum[32 * q + 4 * j + 2], sum[32 * q + 4 * j + 3]);
+        __syncwarp();
+        const int n = first + 32 * q + c;
+        if (n >= n_out) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + lane / 8;
+          if (r >= rows) break;
+          float4 v = *reinterpret_cast<const float4 *>(mid + r * PITCH + c);
+          const long long at = (long long)(m0 + r) * p.ldo + n;
+          if (vector && n + 4 <= n_out) {
+            if (EPI == EPI_BF16) {
+              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+              *reinterpret_cast<uint2 *>(static_cast<bf16 *>(p.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+            } else {
+              float *to = static_cast<float *>(p.out) + at;
+              if (EPI == EPI_ADD_F32) {
+                const float4 old = *reinterpret_cast<const float4 *>(to);
+                v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
+              }
+              *reinterpret_cast<float4 *>(to) = v;
+            }
+          } else {
+            const float each[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (n + e >= n_out) break;
+              if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at + e] = __float2bfloat16_rn(each[e]);
+              else static_cast<float *>(p.out)[at + e] = EPI == EPI_ADD_F32 ? static_cast<float *>(p.out)[at + e] + each[e] : each[e];
+            }
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();                                    // neither CTA's products, copies and arrivals meet a peer that is gone
+  if (warp == ADDERS + 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 2 * BN);
+  }
+}
+
+// How many pairs the device holds at once.
+template <int EPI, bool GROUPED>
+static int most_pairs() {
+  static G2bPerDevice kept;
+  const int dev = g2b_current_device();
+  if (dev >= 0 && kept.value[dev] > 0) return kept.value[dev];
+  const int smem = GROUPED ? SMEM_GROUPED : SMEM;
+  if (cudaFuncSetAttribute(gemm_fp8_tc_kernel<EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, gemm_fp8_tc_kernel<EPI, GROUPED>, &cfg) != cudaSuccess) n = 0;
+  if (dev >= 0) kept.value[dev] = n;
+  return n;
+}
+
+template <int EPI, bool GROUPED>
+static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Tc &p, cudaStream_t stream) {
+  const int most = most_pairs<EPI, GROUPED>();
+  if (most < 1) G2B_REFUSE("gemm_fp8_tc: the device holds no pair with %d bytes of shared memory", GROUPED ? SMEM_GROUPED : SMEM);
+  const long long tiles_n = (p.N + BN - 1) / BN;
+  const long long tiles = GROUPED ? most : ((long long)p.M + 2 * BM - 1) / (2 * BM) * tiles_n;
+  if (((long long)p.M / (2 * BM) + 1 + (GROUPED ? p.n_experts : 0)) * tiles_n > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %d x %d is too large for one launch", p.M, p.N);
+  const int pairs = (int)(tiles < most ? tiles : most);
+  g2b_launch_cluster(gemm_fp8_tc_kernel<EPI, GROUPED>, dim3(2 * pairs), dim3(THREADS), (size_t)(GROUPED ? SMEM_GROUPED : SMEM), stream, 2u, map_a, map_w, p);
+  return g2b_check_launch("gemm_fp8_tc");
+}
+
+// As g2b_gemm_fp8 (gemm_fp8.cu); with EPI_GATED_ROWS out is e4m3 [M, ldo] and out_scale float [ceil(N / 256), ldos].
+extern "C" int g2b_gemm_fp8_tc(const void *a, const float *sa, const void *w, const float *sw, void *out, float *out_scale, int M, int N, int blocks,
+                               long long lda, long long lds, long long ldw, long long ldo, long long ldos, int epi, float limit, float offset, float c1,
+                               float c3, const int *starts, int n_experts, int *status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || blocks <= 0) return 0;
+  if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_tc: rows must start on 16 bytes");
+  const bool gated = epi >= EPI_GATED_F32;
+  if (gated && N % 16) G2B_REFUSE("gemm_fp8_tc: gates and ups in eights, got %d rows", N);
+  if (epi == EPI_GATED_ROWS && (ldo % 16 || ((uintptr_t)out & 15))) G2B_REFUSE("gemm_fp8_tc: quantised rows must start on 16 bytes");
+  if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_tc: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
+  const long long w_rows = (long long)N * (starts ? n_experts : 1);
+  if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %lld rows of W are too many", w_rows);
+  CUtensorMap map_a, map_w;
+  int rc = get_map(&map_a, a, M, blocks * BK, (int)lda, BM, 1);
+  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, BM, 1);
+  if (rc) G2B_REFUSE("gemm_fp8_tc: cuTensorMapEncodeTiled failed (%d)", rc);
+  Tc p;
+  p.sa = sa, p.sw = sw, p.out = out, p.out_scale = out_scale, p.starts = starts, p.status = status;
+  p.M = M, p.N = N, p.blocks = blocks, p.n_experts = n_experts, p.nb = ((gated ? N / 2 : N) + F8_BLOCK - 1) / F8_BLOCK;
+  p.lds = lds, p.ldo = ldo, p.ldos = ldos;
+  p.form.limit = limit, p.form.offset = offset, p.form.c1 = c1, p.form.c3 = c3;
+  if (starts) {
+    switch (epi) {
+      case EPI_F32: return launch<EPI_F32, true>(map_a, map_w, p, stream);
+      case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, true>(map_a, map_w, p, stream);
+    }
+  } else {
+    switch (epi) {
+      case EPI_BF16: return launch<EPI_BF16, false>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<EPI_F32, false>(map_a, map_w, p, stream);
+      case EPI_ADD_F32: return launch<EPI_ADD_F32, false>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<EPI_GATED_F32, false>(map_a, map_w, p, stream);
+      case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, false>(map_a, map_w, p, stream);
+    }
+  }
+  G2B_REFUSE("gemm_fp8_tc: no epilogue %d%s", epi, starts ? " for experts" : "");
+}

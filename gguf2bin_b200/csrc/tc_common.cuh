@@ -378,7 +378,7 @@ struct MapKeyHash {
   }
 };
 
-// A tiled map of a row-major [rows, cols] matrix of bfloat16 (elem_bytes 2) or float (4), row
+// A tiled map of a row-major [rows, cols] matrix of bytes (elem_bytes 1), bfloat16 (2) or float (4), row
 // stride ld elements, with boxes of box_rows rows x 128 bytes and 128-byte swizzle; parts of a
 // box outside the matrix read as zero and are not written.  Encoded maps are kept by (address,
 // sizes): weights, cache layers and scratch buffers come back with the same values every step.
@@ -400,7 +400,9 @@ static inline int get_map(CUtensorMap *map, const void *base, long long rows, in
   cuuint64_t strides[1] = {(cuuint64_t)ld * (cuuint64_t)elem_bytes};
   cuuint32_t box[2] = {(cuuint32_t)(128 / elem_bytes), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+  CUresult r = fn(map, elem_bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                       : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
                   const_cast<void *>(base), dims, strides,
                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

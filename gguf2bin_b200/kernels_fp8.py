@@ -7,12 +7,13 @@ from typing import Optional
 import torch
 
 from . import kernels
+from .kernels_bf16 import _status_word
 from .kernels import SILU, Fp8Matrices, Fp8Matrix, Fp8Rows, KernelError, _call, _code, _fn, _ptr, _stream
 
 BLOCK = 128                          # values of a row, and of either side of a matrix, that share a scale
 F8 = torch.float8_e4m3fn
 MOST_EXPERTS = 1024                  # csrc/quant_fp8.cu
-EPI_BF16, EPI_F32, EPI_ADD_F32, EPI_GATED_F32 = 0, 1, 2, 3
+EPI_BF16, EPI_F32, EPI_ADD_F32, EPI_GATED_F32, EPI_GATED_ROWS = 0, 1, 2, 3, 4
 _FORM = [c_float] * 4
 
 
@@ -152,8 +153,33 @@ def side_by_side(matrices):
 
 
 # ---- products --------------------------------------------------------------------------------------------------
-def _product(rows: Fp8Rows, w: Fp8Matrix, out: torch.Tensor, epi: int, form=SILU, starts=None) -> None:
+def _product_tc(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, defines=()) -> None:
+    """``out``: a tensor, or ``Fp8Rows`` with ``EPI_GATED_ROWS``."""
+    as_rows = epi == EPI_GATED_ROWS
+    to, scale = out if as_rows else (out, None)
+    if workspace is not None:
+        workspace.waits = True
+    f = _fn("gemm_fp8_tc.cu", "g2b_gemm_fp8_tc",
+            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong,
+             c_longlong, c_int, *_FORM, c_void_p, c_int, c_void_p, c_void_p], defines=tuple(defines))
+    _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(to), _ptr(scale), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
+          rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], to.stride(0), scale.stride(0) if as_rows else 0, epi, *form, _ptr(starts),
+          w.q.shape[0] if starts is not None else 0, _ptr(_status_word(to.device)), _stream())
+
+
+MANY_ROWS = 128                      # rows up to which a product goes to the kernel of small tiles
+
+
+def _product(rows: Fp8Rows, w: Fp8Matrix, out: torch.Tensor, epi: int, form=SILU, starts=None, workspace=None) -> None:
     stacked = starts is not None
+    if rows.q.shape[0] > MANY_ROWS * (w.q.shape[0] if stacked else 1):
+        return _product_tc(rows, w, out, epi, form, starts, workspace)
+    if epi == EPI_GATED_ROWS:
+        n, inter = rows.q.shape[0], w.q.shape[-2] // 2
+        h = torch.empty((n, inter), dtype=torch.float32, device=w.q.device) if workspace is None else \
+            workspace.buffer("fp8.mid", (n, inter), torch.float32)
+        _product(rows, w, h, EPI_GATED_F32, form, starts, workspace)
+        return quantize_rows(h, out)
     f = _fn("gemm_fp8.cu", "g2b_gemm_fp8",
             [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int,
              *_FORM, c_void_p, c_int, c_void_p])
@@ -185,7 +211,7 @@ def linear(a, w, out: torch.Tensor, accumulate: bool, workspace) -> None:
     rows = _quantised("linear", a, w.k, workspace)
     _on_device("linear", rows.q, rows.scale, w.q, w.scale, out)
     if tokens:
-        _product(rows, w, out, EPI_ADD_F32 if accumulate else EPI_F32 if out.dtype == torch.float32 else EPI_BF16)
+        _product(rows, w, out, EPI_ADD_F32 if accumulate else EPI_F32 if out.dtype == torch.float32 else EPI_BF16, workspace=workspace)
 
 
 def gate_up(a, w: Fp8Matrix, mid, form, workspace) -> None:
@@ -203,15 +229,8 @@ def gate_up(a, w: Fp8Matrix, mid, form, workspace) -> None:
             raise KernelError(f"gate_up_fused: a matrix in 8 bits leaves float32 or quantised rows, not {mid.dtype}")
     rows = _quantised("gate_up_fused", a, w.k, workspace)
     _on_device("gate_up_fused", rows.q, rows.scale, w.q, w.scale, mid.q if as_rows else mid)
-    if not tokens:
-        return
-    if as_rows:
-        h = torch.empty((tokens, inter), dtype=torch.float32, device=w.q.device) if workspace is None else \
-            workspace.buffer("fp8.mid", (tokens, inter), torch.float32)
-        _product(rows, w, h, EPI_GATED_F32, form)
-        quantize_rows(h, mid)
-    else:
-        _product(rows, w, mid, EPI_GATED_F32, form)
+    if tokens:
+        _product(rows, w, mid, EPI_GATED_ROWS if as_rows else EPI_GATED_F32, form, workspace=workspace)
 
 
 # ---- experts ---------------------------------------------------------------------------------------------------
@@ -253,11 +272,9 @@ def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down
     moe_sort(idx, n_experts, starts, pair_row)
     rows = new_rows(n_pairs, w_gate_up.k, workspace, "fp8.sorted", h.device)
     quantize_rows(h, rows, pair_row)
-    mid = scratch("fp8.mid", (n_pairs, inter), torch.float32)
-    _product(rows, w_gate_up, mid, EPI_GATED_F32, form, starts)
-    mid_rows = new_rows(n_pairs, inter, workspace, "fp8.mid_rows", h.device)
-    quantize_rows(mid, mid_rows)
-    _product(mid_rows, w_down, rows32, EPI_F32, SILU, starts)
+    mid = new_rows(n_pairs, inter, workspace, "fp8.mid_rows", h.device)
+    _product(rows, w_gate_up, mid, EPI_GATED_ROWS, form, starts, workspace)
+    _product(mid, w_down, rows32, EPI_F32, SILU, starts, workspace)
 
 
 def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool) -> None:

@@ -361,3 +361,27 @@ def test_empty_and_repeated_calls():
     for o in outs:
         kernels.linear(x, w, o)
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("epi", ["store", "rows"])
+def test_products_whose_copies_never_come(epi):
+    """The build whose copy role issues nothing: every wait runs out, the kernel returns and the host learns of it."""
+    from gguf2bin_b200 import kernels, kernels_bf16, kernels_fp8
+    from gguf2bin_b200.csrc.units import WAITS_RUN_OUT
+    kernels_bf16.check_status()
+    x, w = operands(300, 512, 384)
+    rows, out = kernels.Fp8Rows(*held(x)), torch.zeros(300, 512, device=DEV)
+    if epi == "rows":
+        w = kernels.Fp8Matrix(*random_matrix(256, 384, DEV, 1, None, True), 384)
+        kernels_fp8._product_tc(rows, w, new_rows(300, 256), kernels_fp8.EPI_GATED_ROWS, kernels.SILU, None, None, WAITS_RUN_OUT)
+    else:
+        kernels_fp8._product_tc(rows, w, out, kernels_fp8.EPI_F32, kernels.SILU, None, None, WAITS_RUN_OUT)
+    torch.cuda.synchronize()
+    with pytest.raises(kernels.KernelError, match="gemm_fp8_tc.*gave up waiting"):
+        kernels_bf16.check_status()
+    if epi == "store":
+        kernels.linear(rows, w, out)
+        kernels_bf16.check_status()
+        again = torch.empty_like(out)
+        kernels.linear(x, w, again)
+        assert torch.equal(out, again) and out.abs().sum() > 0
