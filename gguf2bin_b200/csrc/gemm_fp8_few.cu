@@ -1,0 +1,353 @@
+// Products in 8-bit floating point (fp8.cuh) of few rows, where the bytes of W are what counts:
+//   C[t, n] = sum_b s[b, t] S[n / 128, b] sum_{k in block b} q[t, k] Q[n, k].
+//
+// A CTA takes 128 rows of W (the M of a tcgen05.mma), NX rows of A (its N: 16, 32, 64 or 128) and a range of the blocks of K; the CTAs of a
+// cluster take the ranges of one tile.  A block's sums are formed in one of NACC accumulators in tensor memory.  Roles by warp:
+//   warps 0 .. 4 ADD - 1   add: a thread owns a row of W and 64 columns at most; it adds a finished accumulator, times the row's and the columns' scales
+//                          (their products are in shared memory, CHUNK blocks at a time), to its sums
+//   the next one           copies: STAGES blocks of W and A in flight.  W does not depend on what the stream ran before, so its first stages are
+//                          asked for before that has ended
+//   the last one           products
+// Behind its range every CTA sends its sums, column by column, to the CTA of the cluster that owns the column; that one adds them in the
+// order of the ranges and writes them, neighbouring lanes neighbouring outputs.  So a result depends on the sizes alone.
+//
+// `starts`: W is a stack of matrices and rows starts[e] .. starts[e + 1] of A meet the e-th.  Gated: rows of W alternate, eight gates and the eight
+// ups of the same outputs, each with the scales of their own matrix.
+//
+// Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
+#include "fp8.cuh"
+#include "glu.cuh"
+#include "tc_common.cuh"
+
+G2B_DEFINE_LAST_ERROR
+
+using namespace tc;
+
+enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3 };
+enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
+
+constexpr int WM = 128, BK = F8_BLOCK, W_BYTES = WM * BK;
+constexpr int CHUNK = 16;                                // blocks whose scales are in shared memory at a time
+constexpr int MOST_EXPERTS = 1024;
+
+template <int NX> struct Shape {
+  static constexpr int ADD = NX == 128 ? 2 : 1;          // groups of four adding warps, 64 columns each at most
+  static constexpr int COLS = NX / ADD;
+  static constexpr int STAGES = NX == 16 ? 5 : NX == 32 ? 4 : NX == 64 ? 6 : 4;       // two CTAs a multiprocessor up to 32 columns, else one
+  static constexpr int NACC = NX <= 32 ? 8 : NX == 64 ? 4 : 2;
+  static constexpr int STAGE_BYTES = W_BYTES + NX * BK;
+  static constexpr int RING = STAGES * STAGE_BYTES, SENT = NX * WM * 4, FACTORS = 2 * CHUNK * NX * 4;
+  static constexpr int SMEM = RING + SENT + FACTORS + 256 + 1024;                     // + barriers, + the swizzle's alignment
+  static constexpr int THREADS = (4 * ADD + 2) * 32;
+  static constexpr int TMEM = NACC * NX;
+};
+static_assert(2 * (Shape<16>::SMEM + 1024) <= 228 * 1024 && 2 * (Shape<32>::SMEM + 1024) <= 228 * 1024, "two CTAs a multiprocessor");
+static_assert(Shape<64>::SMEM <= 227 * 1024 && Shape<128>::SMEM <= 227 * 1024, "one CTA a multiprocessor");
+
+struct Few {
+  const float *sa, *sw;
+  void *out;
+  const int *starts;
+  int *status;
+  int M, N, blocks, n_experts, nb, split;                // nb: blocks of W's rows that have a scale
+  long long lds, ldo;
+  GluForm form;
+};
+
+template <bool ACC>
+__device__ __forceinline__ void umma_f8(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  constexpr uint32_t HIGH = (1024 >> 4) | (1u << 14) | (2u << 29);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}\n"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(HIGH), "n"(ACC ? 1 : 0)
+      : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
+
+#define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+// N columns of this thread's lane, waited for (the registers pass through the wait, so that nothing that reads them moves in front)
+__device__ __forceinline__ void read_columns(uint32_t from, uint32_t (&x)[16]) {
+  tmem_ld16(from, x);
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x, 0), F8_RW8(x, 8) : : "memory");
+}
+__device__ __forceinline__ void read_columns(uint32_t from, uint32_t (&x)[32]) {
+  tmem_ld32(from, x);
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x, 0), F8_RW8(x, 8), F8_RW8(x, 16), F8_RW8(x, 24) : : "memory");
+}
+
+template <int NX, int EPI, bool GROUPED>
+__global__ void __launch_bounds__(Shape<NX>::THREADS)
+gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Few p) {
+  using S = Shape<NX>;
+  constexpr bool GATED = EPI == EPI_GATED_F32;
+  constexpr int ADDERS = 4 * S::ADD, PIECE = S::COLS < 32 ? S::COLS : 32;
+  constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(WM >> 4) << 24);      // accumulator float, operands e4m3, K-major
+  pdl_launch();
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float *sent = reinterpret_cast<float *>(smem + S::RING);                // [range][column owned][row]
+  float *factors = sent + NX * WM;                                        // [gate, up][block of the chunk][column]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(factors + 2 * CHUNK * NX);
+  const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * S::STAGES, sum_full0 = empty0 + 8 * S::STAGES, sum_empty0 = sum_full0 + 8 * S::NACC;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + 2 * S::NACC);
+  int *found = reinterpret_cast<int *>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)(blockIdx.x % p.split), n0 = (int)(blockIdx.x / p.split) * WM;
+  const int per = (p.blocks + p.split - 1) / p.split, kb0 = rank * per, nkb = max(0, min(p.blocks, kb0 + per) - kb0);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < S::NACC; ++b) {
+      mbar_init(sum_full0 + 8 * b, 1);
+      mbar_init(sum_empty0 + 8 * b, ADDERS);
+    }
+    mbar_init_fence();
+  }
+  int e = 0, m0 = (int)blockIdx.y * NX, end = p.M;
+  if (GROUPED) {
+    pdl_wait();
+    if (warp == 0) {                                     // which expert's which rows: tiles of the experts, 32 at a time
+      int left = (int)blockIdx.y, at = -1, row = 0, last = 0;
+      for (int e0 = 0; e0 < p.n_experts && at < 0; e0 += 32) {
+        const int x = e0 + lane, first = x < p.n_experts ? p.starts[x] : 0, behind = x < p.n_experts ? p.starts[x + 1] : 0;
+        const int own = (behind - first + NX - 1) / NX;
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, sum, o);
+          if (lane >= o) sum += v;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, sum > left);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          at = e0 + l;
+          row = __shfl_sync(0xffffffffu, first + (left - (sum - own)) * NX, l);
+          last = __shfl_sync(0xffffffffu, behind, l);
+        } else {
+          left -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+      }
+      if (lane == 0) found[0] = at, found[1] = row, found[2] = last;
+    }
+    __syncthreads();
+    e = found[0], m0 = found[1], end = found[2];
+    if (e < 0) return;                                   // (the whole cluster: its CTAs have one blockIdx.y)
+  }
+  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");      // waited for before the first word is sent: everybody has begun
+  if (warp == ADDERS + 1) tmem_alloc(smem_addr(tmem_slot), S::TMEM);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == ADDERS) {
+    if (lane == 0 && PRODUCER_RUNS) {
+      const int row_w = e * p.N + n0;
+      const int ahead = min(nkb, S::STAGES);
+      for (int i = 0; i < ahead; ++i) {
+        mbar_expect_tx(full0 + 8 * i, S::STAGE_BYTES);
+        tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES), &map_w, (kb0 + i) * BK, row_w, full0 + 8 * i);
+      }
+      if (!GROUPED) pdl_wait();
+      for (int i = 0; i < ahead; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + W_BYTES, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
+      for (int i = ahead; i < nkb; ++i) {
+        const int s = i % S::STAGES;
+        if (!mbar_wait(empty0 + 8 * s, (i / S::STAGES - 1) & 1)) {
+          atomicExch(p.status, ST_PRODUCER_TIMEOUT);
+          break;
+        }
+        const uint32_t to = smem_addr(smem + s * S::STAGE_BYTES);
+        mbar_expect_tx(full0 + 8 * s, S::STAGE_BYTES);
+        tma_load_2d(to, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * s);
+        tma_load_2d(to + W_BYTES, &map_a, (kb0 + i) * BK, m0, full0 + 8 * s);
+      }
+    }
+    __syncwarp();
+  } else if (warp == ADDERS + 1) {
+    if (lane == 0) {
+      for (int i = 0; i < nkb; ++i) {
+        const int s = i % S::STAGES, h = i % S::NACC;
+        if (!mbar_wait(full0 + 8 * s, (i / S::STAGES) & 1) || (i >= S::NACC && !mbar_wait(sum_empty0 + 8 * h, (i / S::NACC - 1) & 1))) {
+          atomicExch(p.status, ST_MMA_TIMEOUT);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t lo = ((smem_addr(smem + s * S::STAGE_BYTES) & 0x3FFFF) >> 4) | 1u << 16;
+        const uint32_t to = tmem + h * NX;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k == 0) umma_f8<false>(to, lo, lo + W_BYTES / 16, IDESC);
+          else umma_f8<true>(to, lo + 2 * k, lo + W_BYTES / 16 + 2 * k, IDESC);
+        }
+        umma_commit(empty0 + 8 * s);
+        umma_commit(sum_full0 + 8 * h);
+      }
+    }
+    __syncwarp();
+  }
+  const int own = NX / p.split;                          // columns of A's rows that this CTA writes
+  if (warp < ADDERS) {
+    if (!GROUPED) pdl_wait();
+    const int row = 32 * (warp % 4) + lane, col0 = S::COLS * (warp / 4);
+    const uint32_t from0 = tmem + ((uint32_t)(32 * (warp % 4)) << 16) + col0;
+    const int n_block = min((GATED ? n0 / 2 : n0) / F8_BLOCK, p.nb - 1);
+    const float *sw = p.sw + ((long long)e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks + kb0;
+    const float *mine = factors + (GATED && (row & 8) ? CHUNK * NX : 0) + col0;
+    float sum[S::COLS];
+#pragma unroll
+    for (int j = 0; j < S::COLS; ++j) sum[j] = 0.f;
+    bool ok = true;                                      // once a wait gave up nothing is waited for any more (the warps still meet at their barriers)
+    for (int i = 0; i < nkb; ++i) {
+      const int h = i % S::NACC;
+      if (i % CHUNK == 0) {
+        if (i) asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
+        const int count = min(CHUNK, nkb - i);
+        for (int x = threadIdx.x; x < count * NX; x += ADDERS * 32) {
+          const int b = i + x / NX, t = m0 + x % NX;
+          const float a = t < p.M ? p.sa[(kb0 + b) * p.lds + t] : 0.f;
+          factors[x] = a * sw[b];
+          if (GATED) factors[CHUNK * NX + x] = a * sw[(long long)p.nb * p.blocks + b];
+        }
+        asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
+      }
+      if (ok) {
+        ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (i / S::NACC) & 1));
+        if (!ok && lane == 0) atomicExch(p.status, ST_ADDER_TIMEOUT);
+      }
+      if (!ok) continue;
+      tc_fence_after();
+      const float *f = mine + i % CHUNK * NX;
+#pragma unroll
+      for (int c = 0; c < S::COLS; c += PIECE) {
+        uint32_t x[PIECE];
+        read_columns(from0 + h * NX + c, x);
+        if (c + PIECE == S::COLS) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sum_empty0 + 8 * h);
+        }
+#pragma unroll
+        for (int j = 0; j < PIECE; j += 4) {
+          const float4 s = *reinterpret_cast<const float4 *>(f + c + j);
+          const float2 u = fma2(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), make_float2(s.x, s.y), make_float2(sum[c + j], sum[c + j + 1]));
+          const float2 v = fma2(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), make_float2(s.z, s.w), make_float2(sum[c + j + 2], sum[c + j + 3]));
+          sum[c + j] = u.x, sum[c + j + 1] = u.y, sum[c + j + 2] = v.x, sum[c + j + 3] = v.y;
+        }
+      }
+    }
+    // column c goes to the CTA that owns it, as range `rank`'s part
+    if (p.split > 1) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    if (p.split == 1) {
+#pragma unroll
+      for (int j = 0; j < S::COLS; ++j) sent[(col0 + j) * WM + row] = sum[j];
+    } else {
+      const uint32_t base = smem_addr(sent);
+#pragma unroll
+      for (int j = 0; j < S::COLS; ++j) {
+        const int c = col0 + j, to = c / own;
+        st_cluster(map_to_cta(base + ((rank * own + c - to * own) * WM + row) * 4, (uint32_t)to), sum[j]);
+      }
+    }
+  } else if (p.split > 1) {
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+  }
+  tc_fence_before();
+  if (p.split == 1) __syncthreads();
+  else cluster_sync_all();
+  if (warp == ADDERS + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::TMEM);
+  }
+  if (warp < ADDERS) {
+    const int t0 = m0 + rank * own, rows = min(own, end - t0);
+    constexpr int OUTS = GATED ? WM / 2 : WM;            // outputs of a row of A
+    const int n = (GATED ? n0 / 2 : n0) + threadIdx.x % OUTS, n_out = GATED ? p.N / 2 : p.N;
+    if (n < n_out) {
+      const int l = threadIdx.x % OUTS, r0 = GATED ? (l >> 3) * 16 + (l & 7) : l;
+      for (int c = threadIdx.x / OUTS; c < rows; c += ADDERS * 32 / OUTS) {
+        float v = sent[c * WM + r0], u = GATED ? sent[c * WM + r0 + 8] : 0.f;
+        for (int s = 1; s < p.split; ++s) {
+          v += sent[(s * own + c) * WM + r0];
+          if (GATED) u += sent[(s * own + c) * WM + r0 + 8];
+        }
+        const long long at = (long long)(t0 + c) * p.ldo + n;
+        if (GATED) static_cast<float *>(p.out)[at] = glu_value(v, u, p.form);
+        else if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at] = __float2bfloat16_rn(v);
+        else if (EPI == EPI_F32) static_cast<float *>(p.out)[at] = v;
+        else static_cast<float *>(p.out)[at] += v;
+      }
+    }
+  }
+}
+
+template <int NX, int EPI, bool GROUPED>
+static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
+  static G2bPerDevice configured;
+  const int dev = g2b_current_device();
+  if (dev < 0 || !configured.value[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX>::SMEM);
+    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX>::SMEM, cudaGetErrorString(e));
+    if (dev >= 0) configured.value[dev] = 1;
+  }
+  const long long tiles_m = ((long long)p.M + NX - 1) / NX + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
+  const long long tiles_n = (p.N + WM - 1) / WM;
+  if (tiles_m > 65535 || tiles_n * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
+  g2b_launch_cluster(gemm_fp8_few_kernel<NX, EPI, GROUPED>, dim3((unsigned)(tiles_n * p.split), (unsigned)tiles_m), dim3(Shape<NX>::THREADS),
+                     (size_t)Shape<NX>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
+  return g2b_check_launch("gemm_fp8_few");
+}
+
+template <int NX>
+static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
+  if (p.starts) {
+    switch (epi) {
+      case EPI_F32: return launch<NX, EPI_F32, true>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, EPI_GATED_F32, true>(map_a, map_w, p, stream);
+    }
+  } else {
+    switch (epi) {
+      case EPI_BF16: return launch<NX, EPI_BF16, false>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<NX, EPI_F32, false>(map_a, map_w, p, stream);
+      case EPI_ADD_F32: return launch<NX, EPI_ADD_F32, false>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, EPI_GATED_F32, false>(map_a, map_w, p, stream);
+    }
+  }
+  G2B_REFUSE("gemm_fp8_few: no epilogue %d%s", epi, p.starts ? " for experts" : "");
+}
+
+// a [M, lda], w [N, ldw] (`starts`: [n_experts, N, ldw]), scales sa [blocks, lds] and sw [ceil(N / 128), blocks] (gated: [2, ceil(N / 256), blocks]; a
+// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side; split: parts of K (1, 2,
+// 4 or 8).
+extern "C" int g2b_gemm_fp8_few(const void *a, const float *sa, const void *w, const float *sw, void *out, int M, int N, int blocks, long long lda,
+                                long long lds, long long ldw, long long ldo, int epi, float limit, float offset, float c1, float c3, const int *starts,
+                                int n_experts, int columns, int split, int *status, cudaStream_t stream) {
+  if (M <= 0 || N <= 0 || blocks <= 0) return 0;
+  if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_few: rows must start on 16 bytes");
+  if (epi == EPI_GATED_F32 && N % 16) G2B_REFUSE("gemm_fp8_few: gates and ups in eights, got %d rows", N);
+  if (split != 1 && split != 2 && split != 4 && split != 8) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
+  if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_few: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
+  const long long w_rows = (long long)N * (starts ? n_experts : 1);
+  if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %lld rows of W are too many", w_rows);
+  CUtensorMap map_a, map_w;
+  int rc = columns > 0 && columns <= 256 ? get_map(&map_a, a, M, blocks * BK, (int)lda, columns, 1) : -1;
+  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, WM, 1);
+  if (rc) G2B_REFUSE("gemm_fp8_few: cuTensorMapEncodeTiled failed (%d)", rc);
+  Few p;
+  p.sa = sa, p.sw = sw, p.out = out, p.starts = starts, p.status = status;
+  p.M = M, p.N = N, p.blocks = blocks, p.n_experts = n_experts, p.nb = ((epi == EPI_GATED_F32 ? N / 2 : N) + F8_BLOCK - 1) / F8_BLOCK, p.split = split;
+  p.lds = lds, p.ldo = ldo;
+  p.form.limit = limit, p.form.offset = offset, p.form.c1 = c1, p.form.c3 = c3;
+  switch (columns) {
+    case 16: return pick<16>(epi, map_a, map_w, p, stream);
+    case 32: return pick<32>(epi, map_a, map_w, p, stream);
+    case 64: return pick<64>(epi, map_a, map_w, p, stream);
+    case 128: return pick<128>(epi, map_a, map_w, p, stream);
+  }
+  G2B_REFUSE("gemm_fp8_few: %d columns", columns);
+}

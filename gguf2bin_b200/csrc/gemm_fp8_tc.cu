@@ -33,15 +33,16 @@ constexpr int ADDERS = 8, THREADS = (ADDERS + 4) * 32;   // the last two warps o
 // Registers: 384 threads start with 168 each (64,512); the adders hold 128 sums and two pieces of an accumulator and take 232, the others
 // keep 40: 256 * 232 + 128 * 40 = 64,512.
 constexpr int ADDER_REGS = 232, OTHER_REGS = 40;
-constexpr int COLS = BN / 2, AT_ONCE = 16;
+constexpr int COLS = BN / 2, AT_ONCE = 32;
 constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-constexpr int PITCH = 36;                                // floats a row of an adder's 32 x 32 outputs on their way to C
-constexpr int OUT_BYTES = ADDERS * 32 * PITCH * 4;
 constexpr int MOST_EXPERTS = 1024;
-constexpr int BAR_BYTES = 256, LIST_BYTES = (MOST_EXPERTS + 1) * 4;
-constexpr int SMEM = RING_BYTES + OUT_BYTES + 1024 + BAR_BYTES;                        // + the swizzle's alignment
-constexpr int SMEM_GROUPED = SMEM + LIST_BYTES;
-static_assert(SMEM_GROUPED <= 227 * 1024, "one CTA a multiprocessor");
+constexpr int BOX_BYTES = 32 * 128;                      // an adder's outputs on their way to C: 32 rows of 128 bytes, swizzled as the ring is
+constexpr int BAR_BYTES = 256, LIST_BYTES = MOST_EXPERTS * 4;
+// Boxes of an adder: two where there is room, so that one is filled while the other is written out.
+template <bool GROUPED> constexpr int BOXES = GROUPED ? 1 : 2;
+template <bool GROUPED>
+constexpr int SMEM = RING_BYTES + ADDERS * BOXES<GROUPED> * BOX_BYTES + BAR_BYTES + (GROUPED ? LIST_BYTES : 0) + 1024;      // + the swizzle's alignment
+static_assert(SMEM<false> <= 227 * 1024 && SMEM<true> <= 227 * 1024, "one CTA a multiprocessor");
 constexpr int BAND = 8;                                  // tiles along M that are walked side by side
 
 struct Tc {
@@ -50,7 +51,7 @@ struct Tc {
   float *out_scale;                                      // EPI_GATED_ROWS: [blocks of the outputs, ldos]
   const int *starts;
   int *status;
-  int M, N, blocks, n_experts, nb;                       // nb: blocks of W's rows that have a scale
+  int M, N, blocks, n_experts, nb, boxes;                // nb: blocks of W's rows that have a scale; boxes: map_out may be used
   long long lds, ldo, ldos;
   GluForm form;
 };
@@ -68,12 +69,10 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
       : "memory");
 }
 // Waits for this thread's loads of tensor memory; the registers pass through, so that nothing that reads them moves in front.
-__device__ __forceinline__ void loaded16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
-                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
+#define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+__device__ __forceinline__ void loaded64(uint32_t (&a)[32], uint32_t (&b)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(a, 0), F8_RW8(a, 8), F8_RW8(a, 16), F8_RW8(a, 24) : : "memory");
+  asm volatile("" : F8_RW8(b, 0), F8_RW8(b, 8), F8_RW8(b, 16), F8_RW8(b, 24));
 }
 // One arrival on a barrier of the pair: this warp's reads of tensor memory are done (they are waited for); it hands over no data.
 __device__ __forceinline__ void arrive_read(uint32_t cluster_bar) {
@@ -106,11 +105,13 @@ __device__ __forceinline__ Tile find_tile(const Tc &p, const int *list, int t, i
 
 template <int EPI, bool GROUPED>
 __global__ void __launch_bounds__(THREADS, 1)
-gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Tc p) {
+gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
+                   const __grid_constant__ Tc p) {
   constexpr bool GATED = EPI == EPI_GATED_F32 || EPI == EPI_GATED_ROWS;
   pdl_launch();
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int OUT_BYTES = ADDERS * BOXES<GROUPED> * BOX_BYTES;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + RING_BYTES + OUT_BYTES);
   const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * STAGES, sum_full0 = empty0 + 8 * STAGES, sum_empty0 = sum_full0 + 16;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 4);
@@ -185,7 +186,7 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       for (int t = pair; t < n_tiles && ok; t += pairs)
         for (int b = 0; b < p.blocks; ++b, ++it) {
           const int s = it % STAGES, h = it & 1;
-          if ((it >= 2 && !mbar_wait_cluster(sum_empty0 + 8 * h, (it / 2 - 1) & 1)) || !mbar_wait(full0 + 8 * s, (it / STAGES) & 1)) {
+          if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1) || (it >= 2 && !mbar_wait(sum_empty0 + 8 * h, (it / 2 - 1) & 1))) {
             atomicExch(p.status, ST_MMA_TIMEOUT);
             ok = false;
             break;
@@ -208,28 +209,33 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const int row0 = 32 * (warp % 4), col0 = COLS * (warp / 4);
     const uint32_t first_empty0 = map_to_cta(sum_empty0, 0);
     const uint32_t from0 = tmem + ((uint32_t)row0 << 16) + col0;
-    float *const mid = reinterpret_cast<float *>(smem + RING_BYTES) + warp * 32 * PITCH;
+    unsigned char *const boxes = smem + RING_BYTES + warp * BOXES<GROUPED> * BOX_BYTES;
+    int box = 0;
     bool ok = true;                                      // once a wait gave up nothing is waited for any more, and (but with EPI_GATED_ROWS, whose warps
     int it = 0;                                          // meet in pairs at every tile) nothing is written
     for (int t = pair; t < n_tiles; t += pairs) {
-      const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
-      const int m0 = tile.m0 + (int)half * BM + row0, row = m0 + lane;
-      const float *sa = p.sa + min(row, p.M - 1);
-      // the scales of the thread's columns: one block of W's rows; gated, one of the gate's and one of the up's
-      const int n_block = GATED ? tile.n0 / 2 / F8_BLOCK : min((tile.n0 + col0) / F8_BLOCK, p.nb - 1);
-      const float *sw = p.sw + ((long long)tile.e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks;
-      const float *sw_up = sw + (long long)p.nb * p.blocks;
+      // Inside the loop over K the sums and the pieces of an accumulator take 192 of the 232 registers, so little else lives there: the tile is
+      // found again behind it, and the scales' places are 32-bit offsets (84 bytes of spills in this loop cost 401 -> 586 us).
+      int at_a, at_w;
+      {
+        const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
+        at_a = min(tile.m0 + (int)half * BM + row0 + lane, p.M - 1);
+        // the thread's columns are one block of W's rows; gated, one of the gate's and one of the up's
+        const int n_block = GATED ? tile.n0 / 2 / F8_BLOCK : min((tile.n0 + col0) / F8_BLOCK, p.nb - 1);
+        at_w = (tile.e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks;
+      }
       float sum[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
-      float next_a = sa[0], next_w = sw[0], next_up = GATED ? sw_up[0] : 0.f;
+      float next_a = p.sa[at_a], next_w = p.sw[at_w], next_up = GATED ? p.sw[at_w + p.nb * p.blocks] : 0.f;
       for (int b = 0; b < p.blocks; ++b, ++it) {
         const int h = it & 1;
         const float f = next_a * next_w, f_up = next_a * next_up;
         if (b + 1 < p.blocks) {
-          next_a = sa[(b + 1) * p.lds];
-          next_w = sw[b + 1];
-          if (GATED) next_up = sw_up[b + 1];
+          at_a += (int)p.lds, ++at_w;
+          next_a = p.sa[at_a];
+          next_w = p.sw[at_w];
+          if (GATED) next_up = p.sw[at_w + p.nb * p.blocks];
         }
         if (!ok) continue;
         ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (it / 2) & 1));      // the warp's lanes agree: its loads are all lanes'
@@ -238,26 +244,36 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           continue;
         }
         tc_fence_after();
+        // Two pieces of 32 columns are asked for at once, and the next two as the first ones are used: two waits a block.
         uint32_t x[2][AT_ONCE];
-        tmem_ld16(from0 + h * BN, x[0]);
-#pragma unroll
-        for (int c = 0; c < COLS; c += AT_ONCE) {
-          const int cur = c / AT_ONCE & 1;
-          loaded16(x[cur]);
-          if (c + AT_ONCE < COLS) tmem_ld16(from0 + h * BN + c + AT_ONCE, x[cur ^ 1]);
+        const uint32_t from = from0 + h * BN;
+        auto add = [&](int c, const uint32_t (&v)[AT_ONCE]) {
 #pragma unroll
           for (int j = 0; j < AT_ONCE; j += 2) {
             const float fj = GATED && (j & 8) ? f_up : f;
-            const float2 v = fma2(make_float2(__uint_as_float(x[cur][j]), __uint_as_float(x[cur][j + 1])), make_float2(fj, fj),
-                                  make_float2(sum[c + j], sum[c + j + 1]));
-            sum[c + j] = v.x, sum[c + j + 1] = v.y;
+            const float2 s = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(fj, fj), make_float2(sum[c + j], sum[c + j + 1]));
+            sum[c + j] = s.x, sum[c + j + 1] = s.y;
           }
-        }
-        tc_fence_before();
+        };
+        tmem_ld32(from, x[0]);
+        tmem_ld32(from + 32, x[1]);
+        loaded64(x[0], x[1]);
+        add(0, x[0]);
+        tmem_ld32(from + 64, x[0]);
+        add(32, x[1]);
+        tmem_ld32(from + 96, x[1]);
+        loaded64(x[0], x[1]);
+        tc_fence_before();                               // the accumulator is read: its next products need not wait for these sums
         __syncwarp();
         if (lane == 0) arrive_read(first_empty0 + 8 * h);
+        add(64, x[0]);
+        add(96, x[1]);
       }
       if (!ok && EPI != EPI_GATED_ROWS) break;
+      int again = t;
+      asm volatile("" : "+r"(again));
+      const Tile tile = find_tile<GROUPED>(p, list, again, tiles_n);
+      const int m0 = tile.m0 + (int)half * BM + row0;
       const int rows = min(32, tile.end - m0);           // of this warp's that exist (may be none)
       if (GATED) {
         const int n_out = p.N / 2, out0 = (tile.n0 + col0) / 2;                        // 64 outputs a thread
@@ -271,14 +287,14 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           most = max_nan(most, fabsf(v));
         }
         if (EPI == EPI_GATED_ROWS) {
-          float *const given = mid;                      // the largest of a row: of the two warps that share it
+          float *const given = reinterpret_cast<float *>(boxes);       // the largest of a row: of the two warps that share it
           given[lane] = most;
           asm volatile("bar.sync %0, 64;\n" ::"r"(1 + warp % 4) : "memory");
-          most = max_nan(most, (mid + (warp < 4 ? 4 : -4) * 32 * PITCH)[lane]);
+          most = max_nan(most, (given + (warp < 4 ? 4 : -4) * BOXES<GROUPED> * BOX_BYTES / 4)[lane]);
           const BlockScale s = block_scale(most);
           if (lane < rows) {
-            if (warp < 4) p.out_scale[tile.n0 / 2 / F8_BLOCK * p.ldos + row] = s.scale;
-            uint8_t *to = static_cast<uint8_t *>(p.out) + row * p.ldo + out0;
+            if (warp < 4) p.out_scale[tile.n0 / 2 / F8_BLOCK * p.ldos + m0 + lane] = s.scale;
+            uint8_t *to = static_cast<uint8_t *>(p.out) + (long long)(m0 + lane) * p.ldo + out0;
 #pragma unroll
             for (int j = 0; j < COLS / 2; j += 16) {
               uint32_t w[4];
@@ -293,51 +309,75 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
       }
       if (rows <= 0) continue;
-      // 32 x 32 outputs at a time through shared memory, eight lanes a row
-      constexpr int OUTS = GATED ? COLS / 2 : COLS;
+      // 32 rows of 128 bytes at a time through a box: written out (or added to what is there: every output gets one addition) by the copy unit,
+      // or, where C's rows do not start on 16 bytes or some of the rows are another expert's, read back by the warp, eight lanes a row.
+      constexpr int OUTS = GATED ? COLS / 2 : COLS, WIDE = EPI == EPI_BF16 ? 64 : 32;
       const int n_out = GATED ? p.N / 2 : p.N, first = GATED ? (tile.n0 + col0) / 2 : tile.n0 + col0;
-      const int c = 4 * (lane % 8);
-      const bool vector = p.ldo % 4 == 0 && ((uintptr_t)p.out & (EPI == EPI_BF16 ? 7 : 15)) == 0;
+      const bool copied = p.boxes && (!GROUPED || rows == 32);
 #pragma unroll
-      for (int q = 0; q < OUTS / 32; ++q) {
+      for (int q = 0; q < OUTS / WIDE; ++q) {
+        const int n0 = first + WIDE * q;
+        if (n0 >= n_out) break;
+        int l = lane;
+        asm volatile("" : "+r"(l));                      // or the boxes' addresses are kept over the loop above
+        unsigned char *const at = boxes + box * BOX_BYTES;
+        box = (box + 1) % BOXES<GROUPED>;
+        if (lane == 0) bulk_wait_read<BOXES<GROUPED> - 1>();
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          *reinterpret_cast<float4 *>(mid + lane * PITCH + 4 * j) =
-              make_float4(sum[32 * q + 4 * j], sum[32 * q + 4 * j + 1], sum[32 * q + 4 * j + 2], sum[32 * q + 4 * j + 3]);
-        __syncwarp();
-        const int n = first + 32 * q + c;
-        if (n >= n_out) continue;
+        for (int j = 0; j < 8; ++j) {
+          const int c = WIDE * q + WIDE / 8 * j;
+          uint4 w;
+          if (EPI == EPI_BF16) {
+            uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = 4 * i + lane / 8;
-          if (r >= rows) break;
-          float4 v = *reinterpret_cast<const float4 *>(mid + r * PITCH + c);
-          const long long at = (long long)(m0 + r) * p.ldo + n;
-          if (vector && n + 4 <= n_out) {
-            if (EPI == EPI_BF16) {
-              const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
-              *reinterpret_cast<uint2 *>(static_cast<bf16 *>(p.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-            } else {
-              float *to = static_cast<float *>(p.out) + at;
-              if (EPI == EPI_ADD_F32) {
-                const float4 old = *reinterpret_cast<const float4 *>(to);
-                v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
-              }
-              *reinterpret_cast<float4 *>(to) = v;
+            for (int i = 0; i < 4; ++i) {
+              const __nv_bfloat162 pair2 = __floats2bfloat162_rn(sum[c + 2 * i], sum[c + 2 * i + 1]);
+              u[i] = *reinterpret_cast<const uint32_t *>(&pair2);
             }
+            w = make_uint4(u[0], u[1], u[2], u[3]);
           } else {
-            const float each[4] = {v.x, v.y, v.z, v.w};
+            w = make_uint4(__float_as_uint(sum[c]), __float_as_uint(sum[c + 1]), __float_as_uint(sum[c + 2]), __float_as_uint(sum[c + 3]));
+          }
+          *reinterpret_cast<uint4 *>(at + l * 128 + ((j ^ (l & 7)) << 4)) = w;
+        }
+        if (copied) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            if (EPI == EPI_ADD_F32) tma_reduce_add_2d(&map_out, smem_addr(at), n0, m0);
+            else tma_store_2d(&map_out, smem_addr(at), n0, m0);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + lane / 8, j = lane % 8, n = n0 + WIDE / 8 * j;
+            if (r >= rows) break;
+            const uint4 w = *reinterpret_cast<const uint4 *>(at + r * 128 + ((j ^ (r & 7)) << 4));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            const long long to = (long long)(m0 + r) * p.ldo + n;
+            if (p.boxes && n + WIDE / 8 <= n_out) {      // (of an expert's last rows; nothing is added to there)
+              *reinterpret_cast<uint4 *>(static_cast<unsigned char *>(p.out) + to * (EPI == EPI_BF16 ? 2 : 4)) = w;
+              continue;
+            }
+#pragma unroll
+            for (int e = 0; e < WIDE / 8; ++e) {
               if (n + e >= n_out) break;
-              if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at + e] = __float2bfloat16_rn(each[e]);
-              else static_cast<float *>(p.out)[at + e] = EPI == EPI_ADD_F32 ? static_cast<float *>(p.out)[at + e] + each[e] : each[e];
+              if (EPI == EPI_BF16) {
+                static_cast<uint16_t *>(p.out)[to + e] = (uint16_t)(u[e / 2] >> 16 * (e & 1));
+              } else {
+                float *one = static_cast<float *>(p.out) + to + e;
+                *one = EPI == EPI_ADD_F32 ? *one + __uint_as_float(u[e]) : __uint_as_float(u[e]);
+              }
             }
           }
+          __syncwarp();
         }
       }
     }
+    if (lane == 0) bulk_wait<0>();                       // what the copy unit still reads and writes
   }
   __syncwarp();
   tc_fence_before();
@@ -354,7 +394,7 @@ static int most_pairs() {
   static G2bPerDevice kept;
   const int dev = g2b_current_device();
   if (dev >= 0 && kept.value[dev] > 0) return kept.value[dev];
-  const int smem = GROUPED ? SMEM_GROUPED : SMEM;
+  const int smem = SMEM<GROUPED>;
   if (cudaFuncSetAttribute(gemm_fp8_tc_kernel<EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = (size_t)smem;
@@ -369,18 +409,25 @@ static int most_pairs() {
 }
 
 template <int EPI, bool GROUPED>
-static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Tc &p, cudaStream_t stream) {
+static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, Tc p, cudaStream_t stream) {
   const int most = most_pairs<EPI, GROUPED>();
-  if (most < 1) G2B_REFUSE("gemm_fp8_tc: the device holds no pair with %d bytes of shared memory", GROUPED ? SMEM_GROUPED : SMEM);
+  if (most < 1) G2B_REFUSE("gemm_fp8_tc: the device holds no pair with %d bytes of shared memory", SMEM<GROUPED>);
   const long long tiles_n = (p.N + BN - 1) / BN;
   const long long tiles = GROUPED ? most : ((long long)p.M + 2 * BM - 1) / (2 * BM) * tiles_n;
   if (((long long)p.M / (2 * BM) + 1 + (GROUPED ? p.n_experts : 0)) * tiles_n > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %d x %d is too large for one launch", p.M, p.N);
   const int pairs = (int)(tiles < most ? tiles : most);
-  g2b_launch_cluster(gemm_fp8_tc_kernel<EPI, GROUPED>, dim3(2 * pairs), dim3(THREADS), (size_t)(GROUPED ? SMEM_GROUPED : SMEM), stream, 2u, map_a, map_w, p);
+  CUtensorMap map_out = map_a;
+  constexpr int SIZE = EPI == EPI_BF16 ? 2 : 4;
+  p.boxes = EPI != EPI_GATED_ROWS && p.ldo * SIZE % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldo <= INT32_MAX;
+  if (p.boxes) {
+    const int rc = get_map(&map_out, p.out, p.M, EPI == EPI_GATED_F32 ? p.N / 2 : p.N, (int)p.ldo, 32, SIZE);
+    if (rc) G2B_REFUSE("gemm_fp8_tc: cuTensorMapEncodeTiled failed (%d)", rc);
+  }
+  g2b_launch_cluster(gemm_fp8_tc_kernel<EPI, GROUPED>, dim3(2 * pairs), dim3(THREADS), (size_t)SMEM<GROUPED>, stream, 2u, map_a, map_w, map_out, p);
   return g2b_check_launch("gemm_fp8_tc");
 }
 
-// As g2b_gemm_fp8 (gemm_fp8.cu); with EPI_GATED_ROWS out is e4m3 [M, ldo] and out_scale float [ceil(N / 256), ldos].
+// As g2b_gemm_fp8_few (gemm_fp8_few.cu); with EPI_GATED_ROWS out is e4m3 [M, ldo] and out_scale float [ceil(N / 256), ldos].
 extern "C" int g2b_gemm_fp8_tc(const void *a, const float *sa, const void *w, const float *sw, void *out, float *out_scale, int M, int N, int blocks,
                                long long lda, long long lds, long long ldw, long long ldo, long long ldos, int epi, float limit, float offset, float c1,
                                float c3, const int *starts, int n_experts, int *status, cudaStream_t stream) {
@@ -391,7 +438,7 @@ extern "C" int g2b_gemm_fp8_tc(const void *a, const float *sa, const void *w, co
   if (epi == EPI_GATED_ROWS && (ldo % 16 || ((uintptr_t)out & 15))) G2B_REFUSE("gemm_fp8_tc: quantised rows must start on 16 bytes");
   if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_tc: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
   const long long w_rows = (long long)N * (starts ? n_experts : 1);
-  if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %lld rows of W are too many", w_rows);
+  if ((w_rows / F8_BLOCK + 2ll * n_experts + 2) * blocks > INT32_MAX || w_rows > INT32_MAX || lds * blocks > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %d rows of A and %lld of W with %d blocks are too many for one launch", M, w_rows, blocks);
   CUtensorMap map_a, map_w;
   int rc = get_map(&map_a, a, M, blocks * BK, (int)lda, BM, 1);
   if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, BM, 1);

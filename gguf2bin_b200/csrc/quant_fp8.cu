@@ -112,7 +112,7 @@ extern "C" int g2b_quantize_rows(const void *x, int dtype, long long x_stride, i
 template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_matrix_kernel(const T *__restrict__ w, int N, int K, long long w_stride, uint8_t *__restrict__ q, long long q_stride, float *__restrict__ scale) {
-  pdl_launch();
+  // (no early start for what follows: a product reads its matrix before it waits for the kernel in front of it)
   __shared__ float most[8];
   const int kb = blockIdx.x, nb = blockIdx.y;
   const long long e = blockIdx.z;

@@ -167,25 +167,44 @@ def _product_tc(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, worksp
           w.q.shape[0] if starts is not None else 0, _ptr(_status_word(to.device)), _stream())
 
 
-MANY_ROWS = 128                      # rows up to which a product goes to the kernel of small tiles
+def _product_few(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, columns: int, split: int, defines=()) -> None:
+    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile, K in ``split`` (1, 2, 4 or 8) parts."""
+    if workspace is not None:
+        workspace.waits = True
+    f = _fn("gemm_fp8_few.cu", "g2b_gemm_fp8_few",
+            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int, *_FORM,
+             c_void_p, c_int, c_int, c_int, c_void_p, c_void_p], defines=tuple(defines))
+    _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(out), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
+          rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], out.stride(0), epi, *form, _ptr(starts), w.q.shape[0] if starts is not None else 0,
+          columns, split, _ptr(_status_word(out.device)), _stream())
+
+
+MANY_ROWS = 128                      # rows (of an expert, on average) up to which a product goes to the kernel of few rows
+
+
+def few_shape(rows: int, n: int, blocks: int, experts: int = 0) -> tuple:
+    """(columns, parts of K) of the kernel of few rows."""
+    each = -(-rows // experts) if experts else rows
+    columns = next((c for c in (16, 32, 64) if each <= c), 128)
+    tiles = -(-n // 128) * (min(experts, rows) if experts else -(-rows // columns))
+    most = 296 if columns <= 32 else 148           # CTAs that are there at once
+    split = 1
+    while split < 8 and tiles * split * 2 <= most and blocks >= 4 * split:
+        split *= 2
+    return columns, split
 
 
 def _product(rows: Fp8Rows, w: Fp8Matrix, out: torch.Tensor, epi: int, form=SILU, starts=None, workspace=None) -> None:
-    stacked = starts is not None
-    if rows.q.shape[0] > MANY_ROWS * (w.q.shape[0] if stacked else 1):
+    stacked, n = starts is not None, rows.q.shape[0]
+    if n > MANY_ROWS * (w.q.shape[0] if stacked else 1):
         return _product_tc(rows, w, out, epi, form, starts, workspace)
     if epi == EPI_GATED_ROWS:
-        n, inter = rows.q.shape[0], w.q.shape[-2] // 2
+        inter = w.q.shape[-2] // 2
         h = torch.empty((n, inter), dtype=torch.float32, device=w.q.device) if workspace is None else \
             workspace.buffer("fp8.mid", (n, inter), torch.float32)
         _product(rows, w, h, EPI_GATED_F32, form, starts, workspace)
         return quantize_rows(h, out)
-    f = _fn("gemm_fp8.cu", "g2b_gemm_fp8",
-            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int,
-             *_FORM, c_void_p, c_int, c_void_p])
-    _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(out), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
-          rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], out.stride(0), epi, *form, _ptr(starts), w.q.shape[0] if stacked else 0,
-          _stream())
+    _product_few(rows, w, out, epi, form, starts, workspace, *few_shape(n, w.q.shape[-2], blocks_of(w.k), w.q.shape[0] if stacked else 0))
 
 
 def _check_out(what: str, out: torch.Tensor, rows: int, columns: int) -> None:

@@ -363,25 +363,52 @@ def test_empty_and_repeated_calls():
     assert all(torch.equal(o, outs[0]) for o in outs)
 
 
-@pytest.mark.parametrize("epi", ["store", "rows"])
-def test_products_whose_copies_never_come(epi):
+@pytest.mark.parametrize("kernel", ["tc store", "tc rows", "few", "few parts"])
+def test_products_whose_copies_never_come(kernel):
     """The build whose copy role issues nothing: every wait runs out, the kernel returns and the host learns of it."""
-    from gguf2bin_b200 import kernels, kernels_bf16, kernels_fp8
+    from gguf2bin_b200 import kernels, kernels_bf16
+    from gguf2bin_b200 import kernels_fp8 as K8
     from gguf2bin_b200.csrc.units import WAITS_RUN_OUT
     kernels_bf16.check_status()
-    x, w = operands(300, 512, 384)
-    rows, out = kernels.Fp8Rows(*held(x)), torch.zeros(300, 512, device=DEV)
-    if epi == "rows":
-        w = kernels.Fp8Matrix(*random_matrix(256, 384, DEV, 1, None, True), 384)
-        kernels_fp8._product_tc(rows, w, new_rows(300, 256), kernels_fp8.EPI_GATED_ROWS, kernels.SILU, None, None, WAITS_RUN_OUT)
+    M = 300 if kernel.startswith("tc") else 20
+    x, w = operands(M, 512, 1024)
+    rows, out = kernels.Fp8Rows(*held(x)), torch.zeros(M, 512, device=DEV)
+    if kernel == "tc rows":
+        gated = kernels.Fp8Matrix(*random_matrix(256, 1024, DEV, 1, None, True), 1024)
+        K8._product_tc(rows, gated, new_rows(M, 256), K8.EPI_GATED_ROWS, kernels.SILU, None, None, WAITS_RUN_OUT)
+    elif kernel == "tc store":
+        K8._product_tc(rows, w, out, K8.EPI_F32, kernels.SILU, None, None, WAITS_RUN_OUT)
     else:
-        kernels_fp8._product_tc(rows, w, out, kernels_fp8.EPI_F32, kernels.SILU, None, None, WAITS_RUN_OUT)
+        K8._product_few(rows, w, out, K8.EPI_F32, kernels.SILU, None, None, 32, 1 if kernel == "few" else 4, WAITS_RUN_OUT)
     torch.cuda.synchronize()
-    with pytest.raises(kernels.KernelError, match="gemm_fp8_tc.*gave up waiting"):
+    with pytest.raises(kernels.KernelError, match="gemm_fp8.*gave up waiting"):
         kernels_bf16.check_status()
-    if epi == "store":
-        kernels.linear(rows, w, out)
-        kernels_bf16.check_status()
-        again = torch.empty_like(out)
-        kernels.linear(x, w, again)
-        assert torch.equal(out, again) and out.abs().sum() > 0
+    kernels.linear(rows, w, out)
+    kernels_bf16.check_status()
+    again = torch.empty_like(out)
+    kernels.linear(x, w, again)
+    assert torch.equal(out, again) and out.abs().sum() > 0
+
+
+@pytest.mark.parametrize("columns", [16, 32, 64, 128])
+@pytest.mark.parametrize("split", [1, 2, 4, 8])
+@pytest.mark.parametrize("M,N,K", [(1, 130, 300), (13, 128, 1024), (40, 300, 2176), (150, 200, 640), (5, 64, 5000)])
+def test_every_shape_of_few_rows(M, N, K, columns, split):
+    """Each width and number of parts, ranges of K that are empty or of several chunks of scales, several tiles of rows."""
+    from gguf2bin_b200 import kernels, kernels_bf16
+    from gguf2bin_b200 import kernels_fp8 as K8
+    x, w = operands(M, N, K)
+    rows = kernels.Fp8Rows(*held(x))
+    a, m = rows_values(*rows), matrix_values(w.q, w.scale)
+    out = torch.full((M, N), math.nan, device=DEV)
+    K8._product_few(rows, w, out, K8.EPI_F32, kernels.SILU, None, None, columns, split)
+    kernels_bf16.check_status()
+    assert ((out.double() - a @ m.T).abs() <= (sum_bound(blocks_of(K)) + 8 * EPS) * (a.abs() @ m.abs().T) + 1e-44).all()
+    g = kernels.Fp8Matrix(*random_matrix(N // 16 * 8, K, DEV, 5, None, True), K)
+    g = g._replace(scale=g.scale / math.sqrt(K))
+    x = rnd(M, K, seed=M, dtype=torch.bfloat16)
+    ref, bound = gated_reference(rows_values(*held(x)), g, FORMS["silu"])
+    mid = torch.full((M, N // 16 * 8), math.nan, device=DEV)
+    K8._product_few(kernels.Fp8Rows(*held(x)), g, mid, K8.EPI_GATED_F32, kernels.SILU, None, None, columns, split)
+    kernels_bf16.check_status()
+    assert ((mid.double() - ref).abs() <= bound).all()
