@@ -27,22 +27,22 @@ enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3 };
 enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
 
 constexpr int WM = 128, BK = F8_BLOCK, W_BYTES = WM * BK;
-constexpr int CHUNK = 16;                                // blocks whose scales are in shared memory at a time
 constexpr int MOST_EXPERTS = 1024;
 
+// Two CTAs a multiprocessor (with 128 columns, one).
 template <int NX> struct Shape {
   static constexpr int ADD = NX == 128 ? 2 : 1;          // groups of four adding warps, 64 columns each at most
   static constexpr int COLS = NX / ADD;
-  static constexpr int STAGES = NX == 16 ? 5 : NX == 32 ? 4 : NX == 64 ? 6 : 4;       // two CTAs a multiprocessor up to 32 columns, else one
-  static constexpr int NACC = NX <= 32 ? 8 : NX == 64 ? 4 : 2;
+  static constexpr int STAGES = NX == 16 ? 6 : NX == 32 ? 5 : NX == 64 ? 4 : 6;
+  static constexpr int NACC = NX <= 32 ? 8 : 4;
+  static constexpr int CHUNK = NX <= 32 ? 16 : 8;        // blocks whose scales are in shared memory at a time
   static constexpr int STAGE_BYTES = W_BYTES + NX * BK;
-  static constexpr int RING = STAGES * STAGE_BYTES, SENT = NX * WM * 4, FACTORS = 2 * CHUNK * NX * 4;
-  static constexpr int SMEM = RING + SENT + FACTORS + 256 + 1024;                     // + barriers, + the swizzle's alignment
-  static constexpr int THREADS = (4 * ADD + 2) * 32;
+  static constexpr int RING = STAGES * STAGE_BYTES, SENT = (NX + 4 * 8) * WM * 4, FACTORS = 2 * CHUNK * NX * 4;     // SENT lies where the ring was
+  static constexpr int SMEM = RING + FACTORS + 256 + 1024;                            // + barriers, + the swizzle's alignment
+  static constexpr int THREADS = (4 * ADD + 2) * 32, PER_SM = NX == 128 ? 1 : 2;
   static constexpr int TMEM = NACC * NX;
+  static_assert(SENT <= RING && PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * TMEM <= 512, "what a multiprocessor holds");
 };
-static_assert(2 * (Shape<16>::SMEM + 1024) <= 228 * 1024 && 2 * (Shape<32>::SMEM + 1024) <= 228 * 1024, "two CTAs a multiprocessor");
-static_assert(Shape<64>::SMEM <= 227 * 1024 && Shape<128>::SMEM <= 227 * 1024, "one CTA a multiprocessor");
 
 struct Few {
   const float *sa, *sw;
@@ -66,31 +66,41 @@ __device__ __forceinline__ void umma_f8(uint32_t d, uint32_t a_lo, uint32_t b_lo
       ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(HIGH), "n"(ACC ? 1 : 0)
       : "memory");
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ void st_cluster(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
 
 #define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
-// N columns of this thread's lane, waited for (the registers pass through the wait, so that nothing that reads them moves in front)
-__device__ __forceinline__ void read_columns(uint32_t from, uint32_t (&x)[16]) {
-  tmem_ld16(from, x);
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x, 0), F8_RW8(x, 8) : : "memory");
+// Columns of this thread's lane: asked for, and waited for (the registers pass through the wait, so that nothing that reads them moves in front).
+__device__ __forceinline__ void ask_columns(uint32_t from, uint32_t (&x)[1][16]) { tmem_ld16(from, x[0]); }
+__device__ __forceinline__ void ask_columns(uint32_t from, uint32_t (&x)[1][32]) { tmem_ld32(from, x[0]); }
+__device__ __forceinline__ void ask_columns(uint32_t from, uint32_t (&x)[2][32]) {
+  tmem_ld32(from, x[0]);
+  tmem_ld32(from + 32, x[1]);
 }
-__device__ __forceinline__ void read_columns(uint32_t from, uint32_t (&x)[32]) {
-  tmem_ld32(from, x);
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x, 0), F8_RW8(x, 8), F8_RW8(x, 16), F8_RW8(x, 24) : : "memory");
+__device__ __forceinline__ void got_columns(uint32_t (&x)[1][16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x[0], 0), F8_RW8(x[0], 8) : : "memory");
+}
+__device__ __forceinline__ void got_columns(uint32_t (&x)[1][32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x[0], 0), F8_RW8(x[0], 8), F8_RW8(x[0], 16), F8_RW8(x[0], 24) : : "memory");
+}
+__device__ __forceinline__ void got_columns(uint32_t (&x)[2][32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(x[0], 0), F8_RW8(x[0], 8), F8_RW8(x[0], 16), F8_RW8(x[0], 24) : : "memory");
+  asm volatile("" : F8_RW8(x[1], 0), F8_RW8(x[1], 8), F8_RW8(x[1], 16), F8_RW8(x[1], 24));
 }
 
 template <int NX, int EPI, bool GROUPED>
-__global__ void __launch_bounds__(Shape<NX>::THREADS)
+__global__ void __launch_bounds__(Shape<NX>::THREADS, Shape<NX>::PER_SM)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Few p) {
   using S = Shape<NX>;
   constexpr bool GATED = EPI == EPI_GATED_F32;
-  constexpr int ADDERS = 4 * S::ADD, PIECE = S::COLS < 32 ? S::COLS : 32;
+  constexpr int ADDERS = 4 * S::ADD, CHUNK = S::CHUNK, PIECE = S::COLS < 32 ? S::COLS : 32, PIECES = S::COLS / PIECE;
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(WM >> 4) << 24);      // accumulator float, operands e4m3, K-major
   pdl_launch();
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float *sent = reinterpret_cast<float *>(smem + S::RING);                // [range][column owned][row]
-  float *factors = sent + NX * WM;                                        // [gate, up][block of the chunk][column]
+  float4 *sent = reinterpret_cast<float4 *>(smem);                        // [range][four columns owned][row], behind the loop
+  float *factors = reinterpret_cast<float *>(smem + S::RING);             // [gate, up][block of the chunk][column]
   uint64_t *bars = reinterpret_cast<uint64_t *>(factors + 2 * CHUNK * NX);
   const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * S::STAGES, sum_full0 = empty0 + 8 * S::STAGES, sum_empty0 = sum_full0 + 8 * S::NACC;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + 2 * S::NACC);
@@ -139,7 +149,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     e = found[0], m0 = found[1], end = found[2];
     if (e < 0) return;                                   // (the whole cluster: its CTAs have one blockIdx.y)
   }
-  if (p.split > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");      // waited for before the first word is sent: everybody has begun
   if (warp == ADDERS + 1) tmem_alloc(smem_addr(tmem_slot), S::TMEM);
   tc_fence_before();
   __syncthreads();
@@ -191,7 +200,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
     __syncwarp();
   }
-  const int own = NX / p.split;                          // columns of A's rows that this CTA writes
+  const int own = (NX / 4 + p.split - 1) / p.split * 4;  // columns (rows of A) that a CTA writes, four at a time; the last ones maybe fewer, or none
   if (warp < ADDERS) {
     if (!GROUPED) pdl_wait();
     const int row = 32 * (warp % 4) + lane, col0 = S::COLS * (warp / 4);
@@ -202,19 +211,30 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     float sum[S::COLS];
 #pragma unroll
     for (int j = 0; j < S::COLS; ++j) sum[j] = 0.f;
+    constexpr int PER = CHUNK * NX / (ADDERS * 32);
+    float next_a[PER], next_w[PER], next_up[PER];
+    auto ask = [&](int first) {                          // the scales of a chunk that the thread brings, all at once
+#pragma unroll
+      for (int x = 0; x < PER; ++x) {
+        const int at = threadIdx.x + x * ADDERS * 32, b = min(first + at / NX, nkb - 1), t = m0 + at % NX;
+        next_a[x] = t < p.M ? p.sa[(kb0 + b) * p.lds + t] : 0.f;
+        next_w[x] = sw[b];
+        next_up[x] = GATED ? sw[(long long)p.nb * p.blocks + b] : 0.f;
+      }
+    };
+    if (nkb > 0) ask(0);
     bool ok = true;                                      // once a wait gave up nothing is waited for any more (the warps still meet at their barriers)
     for (int i = 0; i < nkb; ++i) {
       const int h = i % S::NACC;
-      if (i % CHUNK == 0) {
+      if (i % CHUNK == 0) {                              // this chunk's scales are in registers: to shared memory, and the next chunk's asked for
         if (i) asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
-        const int count = min(CHUNK, nkb - i);
-        for (int x = threadIdx.x; x < count * NX; x += ADDERS * 32) {
-          const int b = i + x / NX, t = m0 + x % NX;
-          const float a = t < p.M ? p.sa[(kb0 + b) * p.lds + t] : 0.f;
-          factors[x] = a * sw[b];
-          if (GATED) factors[CHUNK * NX + x] = a * sw[(long long)p.nb * p.blocks + b];
+#pragma unroll
+        for (int x = 0; x < PER; ++x) {
+          factors[threadIdx.x + x * ADDERS * 32] = next_a[x] * next_w[x];
+          if (GATED) factors[CHUNK * NX + threadIdx.x + x * ADDERS * 32] = next_a[x] * next_up[x];
         }
         asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
+        if (i + CHUNK < nkb) ask(i + CHUNK);
       }
       if (ok) {
         ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (i / S::NACC) & 1));
@@ -223,39 +243,41 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       if (!ok) continue;
       tc_fence_after();
       const float *f = mine + i % CHUNK * NX;
+uint32_t x[PIECES][PIECE];
+      ask_columns(from0 + h * NX, x);
+      got_columns(x);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sum_empty0 + 8 * h);
 #pragma unroll
-      for (int c = 0; c < S::COLS; c += PIECE) {
-        uint32_t x[PIECE];
-        read_columns(from0 + h * NX + c, x);
-        if (c + PIECE == S::COLS) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sum_empty0 + 8 * h);
-        }
-#pragma unroll
-        for (int j = 0; j < PIECE; j += 4) {
-          const float4 s = *reinterpret_cast<const float4 *>(f + c + j);
-          const float2 u = fma2(make_float2(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), make_float2(s.x, s.y), make_float2(sum[c + j], sum[c + j + 1]));
-          const float2 v = fma2(make_float2(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), make_float2(s.z, s.w), make_float2(sum[c + j + 2], sum[c + j + 3]));
-          sum[c + j] = u.x, sum[c + j + 1] = u.y, sum[c + j + 2] = v.x, sum[c + j + 3] = v.y;
-        }
+      for (int c = 0; c < S::COLS; c += 4) {
+        const uint32_t *v = &x[c / PIECE][c % PIECE];
+        const float4 s = *reinterpret_cast<const float4 *>(f + c);
+        const float2 u0 = fma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), make_float2(s.x, s.y), make_float2(sum[c], sum[c + 1]));
+        const float2 u1 = fma2(make_float2(__uint_as_float(v[2]), __uint_as_float(v[3])), make_float2(s.z, s.w), make_float2(sum[c + 2], sum[c + 3]));
+        sum[c] = u0.x, sum[c + 1] = u0.y, sum[c + 2] = u1.x, sum[c + 3] = u1.y;
       }
     }
-    // column c goes to the CTA that owns it, as range `rank`'s part
-    if (p.split > 1) asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    // Four columns at a time go to the CTA that owns them, as range `rank`'s part, to where that one's ring was: once the sums of all are complete nobody's
+    // products read a ring any more.
+    if (p.split > 1) cluster_sync_all();
     if (p.split == 1) {
 #pragma unroll
-      for (int j = 0; j < S::COLS; ++j) sent[(col0 + j) * WM + row] = sum[j];
+      for (int j = 0; j < S::COLS; j += 4)
+        sent[(col0 + j) / 4 * WM + row] = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
     } else {
       const uint32_t base = smem_addr(sent);
+      int to = col0 / own, left = own - col0 % own;      // the owner of the columns at hand, and how many of its own are still to come
 #pragma unroll
-      for (int j = 0; j < S::COLS; ++j) {
-        const int c = col0 + j, to = c / own;
-        st_cluster(map_to_cta(base + ((rank * own + c - to * own) * WM + row) * 4, (uint32_t)to), sum[j]);
+      for (int j = 0; j < S::COLS; j += 4) {
+        const uint32_t at = base + ((rank * own + own - left) / 4 * WM + row) * 16;
+        st_cluster(map_to_cta(at, (uint32_t)to), make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]));
+        left -= 4;
+        if (left == 0) ++to, left = own;
       }
     }
   } else if (p.split > 1) {
-    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    cluster_sync_all();
   }
   tc_fence_before();
   if (p.split == 1) __syncthreads();
@@ -265,22 +287,36 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     tmem_dealloc(tmem, S::TMEM);
   }
   if (warp < ADDERS) {
-    const int t0 = m0 + rank * own, rows = min(own, end - t0);
+    const int t0 = m0 + rank * own, rows = min(min(own, NX - rank * own), end - t0);
     constexpr int OUTS = GATED ? WM / 2 : WM;            // outputs of a row of A
     const int n = (GATED ? n0 / 2 : n0) + threadIdx.x % OUTS, n_out = GATED ? p.N / 2 : p.N;
     if (n < n_out) {
       const int l = threadIdx.x % OUTS, r0 = GATED ? (l >> 3) * 16 + (l & 7) : l;
-      for (int c = threadIdx.x / OUTS; c < rows; c += ADDERS * 32 / OUTS) {
-        float v = sent[c * WM + r0], u = GATED ? sent[c * WM + r0 + 8] : 0.f;
-        for (int s = 1; s < p.split; ++s) {
-          v += sent[(s * own + c) * WM + r0];
-          if (GATED) u += sent[(s * own + c) * WM + r0 + 8];
-        }
+      const float4 *from = sent + r0;
+      for (int c = threadIdx.x / OUTS * 4; c < rows; c += ADDERS * 32 / OUTS * 4) {
         const long long at = (long long)(t0 + c) * p.ldo + n;
-        if (GATED) static_cast<float *>(p.out)[at] = glu_value(v, u, p.form);
-        else if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at] = __float2bfloat16_rn(v);
-        else if (EPI == EPI_F32) static_cast<float *>(p.out)[at] = v;
-        else static_cast<float *>(p.out)[at] += v;
+        float4 v = from[c / 4 * WM], u = GATED ? from[c / 4 * WM + 8] : v, old;
+        float *const add = static_cast<float *>(p.out) + at;
+        if (EPI == EPI_ADD_F32)
+          old = make_float4(add[0], c + 1 < rows ? add[p.ldo] : 0.f, c + 2 < rows ? add[2 * p.ldo] : 0.f, c + 3 < rows ? add[3 * p.ldo] : 0.f);
+#pragma unroll
+        for (int s = 1; s < 8; ++s) {
+          if (s >= p.split) break;
+          const float4 x = from[(s * own + c) / 4 * WM];
+          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+          if (GATED) {
+            const float4 y = from[(s * own + c) / 4 * WM + 8];
+            u.x += y.x, u.y += y.y, u.z += y.z, u.w += y.w;
+          }
+        }
+        const float vs[4] = {v.x, v.y, v.z, v.w}, us[4] = {u.x, u.y, u.z, u.w}, olds[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (c + i >= rows) break;
+          if (GATED) static_cast<float *>(p.out)[at + i * p.ldo] = glu_value(vs[i], us[i], p.form);
+          else if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at + i * p.ldo] = __float2bfloat16_rn(vs[i]);
+          else static_cast<float *>(p.out)[at + i * p.ldo] = EPI == EPI_F32 ? vs[i] : olds[i] + vs[i];
+        }
       }
     }
   }
@@ -322,15 +358,15 @@ static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, con
 }
 
 // a [M, lda], w [N, ldw] (`starts`: [n_experts, N, ldw]), scales sa [blocks, lds] and sw [ceil(N / 128), blocks] (gated: [2, ceil(N / 256), blocks]; a
-// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side; split: parts of K (1, 2,
-// 4 or 8).
+// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side; split: parts of K, at
+// most 8.
 extern "C" int g2b_gemm_fp8_few(const void *a, const float *sa, const void *w, const float *sw, void *out, int M, int N, int blocks, long long lda,
                                 long long lds, long long ldw, long long ldo, int epi, float limit, float offset, float c1, float c3, const int *starts,
                                 int n_experts, int columns, int split, int *status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || blocks <= 0) return 0;
   if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_few: rows must start on 16 bytes");
   if (epi == EPI_GATED_F32 && N % 16) G2B_REFUSE("gemm_fp8_few: gates and ups in eights, got %d rows", N);
-  if (split != 1 && split != 2 && split != 4 && split != 8) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
+  if (split < 1 || split > 8) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
   if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_few: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
   const long long w_rows = (long long)N * (starts ? n_experts : 1);
   if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %lld rows of W are too many", w_rows);

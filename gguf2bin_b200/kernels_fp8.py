@@ -168,7 +168,7 @@ def _product_tc(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, worksp
 
 
 def _product_few(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, columns: int, split: int, defines=()) -> None:
-    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile, K in ``split`` (1, 2, 4 or 8) parts."""
+    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile, K in ``split`` parts, at most 8."""
     if workspace is not None:
         workspace.waits = True
     f = _fn("gemm_fp8_few.cu", "g2b_gemm_fp8_few",
