@@ -26,21 +26,36 @@ using namespace tc;
 enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3 };
 enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
 
-constexpr int WM = 128, BK = F8_BLOCK, W_BYTES = WM * BK;
+constexpr int LANES = 128, BK = F8_BLOCK, LANE_BYTES = LANES * BK;
 constexpr int MOST_EXPERTS = 1024;
 
+constexpr int MOST_SPLIT = 8;
+// columns that a CTA of `split` owns, `unit` at a time, and the most that ranges and columns owned come to
+constexpr int columns_owned(int columns, int unit, int split) { return (columns / unit + split - 1) / split * unit; }
+constexpr int most_sent(int columns, int unit) {
+  int most = 0;
+  for (int s = 1; s <= MOST_SPLIT; ++s)
+    if (columns_owned(columns, unit, s) * s > most) most = columns_owned(columns, unit, s) * s;
+  return most;
+}
+
+// LANES_A: the tile the other way round, 128 rows of A on the lanes of tensor memory and NX rows of W as its columns.
 // Two CTAs a multiprocessor (with 128 columns, one).
-template <int NX> struct Shape {
-  static constexpr int ADD = NX == 128 ? 2 : 1;          // groups of four adding warps, 64 columns each at most
+template <int NX, bool LANES_A> struct Shape {
+  static constexpr int ADD = NX >= 64 ? 2 : 1;           // groups of four adding warps, 64 columns each at most
   static constexpr int COLS = NX / ADD;
   static constexpr int STAGES = NX == 16 ? 6 : NX == 32 ? 5 : NX == 64 ? 4 : 6;
-  static constexpr int NACC = NX <= 32 ? 8 : 4;
+  static constexpr int NACC = 4;                         // at most STAGES: a stage's barrier says both that its operands and that its sums are done
   static constexpr int CHUNK = NX <= 32 ? 16 : 8;        // blocks whose scales are in shared memory at a time
-  static constexpr int STAGE_BYTES = W_BYTES + NX * BK;
-  static constexpr int RING = STAGES * STAGE_BYTES, SENT = (NX + 4 * 8) * WM * 4, FACTORS = 2 * CHUNK * NX * 4;     // SENT lies where the ring was
+  static constexpr int PITCH = LANES_A ? LANES + 1 : LANES;                           // of the columns sent: read along rows, or (LANES_A) along columns
+  static constexpr int STAGE_BYTES = LANES * BK + NX * BK;
+  static constexpr int RING = STAGES * STAGE_BYTES, SENT = most_sent(NX, LANES_A ? 16 : 4) / 4 * PITCH * 16;     // SENT lies where the ring was
+  static constexpr int FACTORS = LANES_A ? 0 : 2 * CHUNK * NX * 4;
   static constexpr int SMEM = RING + FACTORS + 256 + 1024;                            // + barriers, + the swizzle's alignment
   static constexpr int THREADS = (4 * ADD + 2) * 32, PER_SM = NX == 128 ? 1 : 2;
   static constexpr int TMEM = NACC * NX;
+  static constexpr int ROWS_A = LANES_A ? LANES : NX, ROWS_W = LANES_A ? NX : LANES;
+  static_assert(NACC <= STAGES, "an adder must have seen a stage's barrier before its next products are issued");
   static_assert(SENT <= RING && PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * TMEM <= 512, "what a multiprocessor holds");
 };
 
@@ -89,44 +104,42 @@ __device__ __forceinline__ void got_columns(uint32_t (&x)[2][32]) {
   asm volatile("" : F8_RW8(x[1], 0), F8_RW8(x[1], 8), F8_RW8(x[1], 16), F8_RW8(x[1], 24));
 }
 
-template <int NX, int EPI, bool GROUPED>
-__global__ void __launch_bounds__(Shape<NX>::THREADS, Shape<NX>::PER_SM)
+template <int NX, bool LANES_A, int EPI, bool GROUPED>
+__global__ void __launch_bounds__(Shape<NX, LANES_A>::THREADS, Shape<NX, LANES_A>::PER_SM)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Few p) {
-  using S = Shape<NX>;
+  using S = Shape<NX, LANES_A>;
   constexpr bool GATED = EPI == EPI_GATED_F32;
   constexpr int ADDERS = 4 * S::ADD, CHUNK = S::CHUNK, PIECE = S::COLS < 32 ? S::COLS : 32, PIECES = S::COLS / PIECE;
-  constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(WM >> 4) << 24);      // accumulator float, operands e4m3, K-major
+  constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(LANES >> 4) << 24);      // accumulator float, operands e4m3, K-major
   pdl_launch();
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float4 *sent = reinterpret_cast<float4 *>(smem);                        // [range][four columns owned][row], behind the loop
   float *factors = reinterpret_cast<float *>(smem + S::RING);             // [gate, up][block of the chunk][column]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(factors + 2 * CHUNK * NX);
-  const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * S::STAGES, sum_full0 = empty0 + 8 * S::STAGES, sum_empty0 = sum_full0 + 8 * S::NACC;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + 2 * S::NACC);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::RING + S::FACTORS);
+  const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * S::STAGES, sum_empty0 = done0 + 8 * S::STAGES;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + S::NACC);
   int *found = reinterpret_cast<int *>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)(blockIdx.x % p.split), n0 = (int)(blockIdx.x / p.split) * WM;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  // (tiles of other rows of A, which read the same W, are neighbours)
+  const int rank = (int)(blockIdx.x % p.split), n0 = (int)blockIdx.y * S::ROWS_W, tile_m = (int)(blockIdx.x / p.split);
   const int per = (p.blocks + p.split - 1) / p.split, kb0 = rank * per, nkb = max(0, min(p.blocks, kb0 + per) - kb0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(full0 + 8 * s, 1);
-      mbar_init(empty0 + 8 * s, 1);
+      mbar_init(done0 + 8 * s, 1);
     }
-    for (int b = 0; b < S::NACC; ++b) {
-      mbar_init(sum_full0 + 8 * b, 1);
-      mbar_init(sum_empty0 + 8 * b, ADDERS);
-    }
+    for (int b = 0; b < S::NACC; ++b) mbar_init(sum_empty0 + 8 * b, ADDERS);
     mbar_init_fence();
   }
-  int e = 0, m0 = (int)blockIdx.y * NX, end = p.M;
+  int e = 0, m0 = tile_m * S::ROWS_A, end = p.M;
   if (GROUPED) {
     pdl_wait();
     if (warp == 0) {                                     // which expert's which rows: tiles of the experts, 32 at a time
-      int left = (int)blockIdx.y, at = -1, row = 0, last = 0;
+      int left = tile_m, at = -1, row = 0, last = 0;
       for (int e0 = 0; e0 < p.n_experts && at < 0; e0 += 32) {
         const int x = e0 + lane, first = x < p.n_experts ? p.starts[x] : 0, behind = x < p.n_experts ? p.starts[x + 1] : 0;
-        const int own = (behind - first + NX - 1) / NX;
+        const int own = (behind - first + S::ROWS_A - 1) / S::ROWS_A;
         int sum = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -137,7 +150,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (hit) {
           const int l = __ffs(hit) - 1;
           at = e0 + l;
-          row = __shfl_sync(0xffffffffu, first + (left - (sum - own)) * NX, l);
+          row = __shfl_sync(0xffffffffu, first + (left - (sum - own)) * S::ROWS_A, l);
           last = __shfl_sync(0xffffffffu, behind, l);
         } else {
           left -= __shfl_sync(0xffffffffu, sum, 31);
@@ -147,7 +160,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
     __syncthreads();
     e = found[0], m0 = found[1], end = found[2];
-    if (e < 0) return;                                   // (the whole cluster: its CTAs have one blockIdx.y)
+    if (e < 0) return;                                   // (the whole cluster: its CTAs have one tile)
   }
   if (warp == ADDERS + 1) tmem_alloc(smem_addr(tmem_slot), S::TMEM);
   tc_fence_before();
@@ -156,51 +169,59 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   const uint32_t tmem = *tmem_slot;
 
   if (warp == ADDERS) {
-    if (lane == 0 && PRODUCER_RUNS) {
-      const int row_w = e * p.N + n0;
+    if (PRODUCER_RUNS) {
+      const int row_w = e * p.N + n0, at_w = LANES_A ? LANE_BYTES : 0, at_a = LANE_BYTES - at_w;
       const int ahead = min(nkb, S::STAGES);
-      for (int i = 0; i < ahead; ++i) {
-        mbar_expect_tx(full0 + 8 * i, S::STAGE_BYTES);
-        tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES), &map_w, (kb0 + i) * BK, row_w, full0 + 8 * i);
+      if (elect_one()) {
+        for (int i = 0; i < ahead; ++i) {
+          mbar_expect_tx(full0 + 8 * i, S::STAGE_BYTES);
+          tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_w, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * i);
+        }
+        if (!GROUPED) pdl_wait();
+        for (int i = 0; i < ahead; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
       }
-      if (!GROUPED) pdl_wait();
-      for (int i = 0; i < ahead; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + W_BYTES, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
+      __syncwarp();
       for (int i = ahead; i < nkb; ++i) {
         const int s = i % S::STAGES;
-        if (!mbar_wait(empty0 + 8 * s, (i / S::STAGES - 1) & 1)) {
-          atomicExch(p.status, ST_PRODUCER_TIMEOUT);
+        if (!__all_sync(0xffffffffu, mbar_wait(done0 + 8 * s, (i / S::STAGES - 1) & 1))) {
+          if (lane == 0) atomicExch(p.status, ST_PRODUCER_TIMEOUT);
           break;
         }
         const uint32_t to = smem_addr(smem + s * S::STAGE_BYTES);
-        mbar_expect_tx(full0 + 8 * s, S::STAGE_BYTES);
-        tma_load_2d(to, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * s);
-        tma_load_2d(to + W_BYTES, &map_a, (kb0 + i) * BK, m0, full0 + 8 * s);
+        if (elect_one()) {
+          mbar_expect_tx(full0 + 8 * s, S::STAGE_BYTES);
+          tma_load_2d(to + at_w, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * s);
+          tma_load_2d(to + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * s);
+        }
+        __syncwarp();
       }
     }
     __syncwarp();
   } else if (warp == ADDERS + 1) {
-    if (lane == 0) {
-      for (int i = 0; i < nkb; ++i) {
-        const int s = i % S::STAGES, h = i % S::NACC;
-        if (!mbar_wait(full0 + 8 * s, (i / S::STAGES) & 1) || (i >= S::NACC && !mbar_wait(sum_empty0 + 8 * h, (i / S::NACC - 1) & 1))) {
-          atomicExch(p.status, ST_MMA_TIMEOUT);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t lo = ((smem_addr(smem + s * S::STAGE_BYTES) & 0x3FFFF) >> 4) | 1u << 16;
-        const uint32_t to = tmem + h * NX;
+    for (int i = 0; i < nkb; ++i) {
+      const int s = i % S::STAGES, h = i % S::NACC;
+      const bool ok = mbar_wait(full0 + 8 * s, (i / S::STAGES) & 1) && (i < S::NACC || mbar_wait(sum_empty0 + 8 * h, (i / S::NACC - 1) & 1));
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) atomicExch(p.status, ST_MMA_TIMEOUT);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t lo = ((smem_addr(smem + s * S::STAGE_BYTES) & 0x3FFFF) >> 4) | 1u << 16;
+      const uint32_t to = tmem + h * NX;
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (k == 0) umma_f8<false>(to, lo, lo + W_BYTES / 16, IDESC);
-          else umma_f8<true>(to, lo + 2 * k, lo + W_BYTES / 16 + 2 * k, IDESC);
+          if (k == 0) umma_f8<false>(to, lo, lo + LANE_BYTES / 16, IDESC);
+          else umma_f8<true>(to, lo + 2 * k, lo + LANE_BYTES / 16 + 2 * k, IDESC);
         }
-        umma_commit(empty0 + 8 * s);
-        umma_commit(sum_full0 + 8 * h);
+        umma_commit(done0 + 8 * s);
       }
+      __syncwarp();
     }
-    __syncwarp();
   }
-  const int own = (NX / 4 + p.split - 1) / p.split * 4;  // columns (rows of A) that a CTA writes, four at a time; the last ones maybe fewer, or none
+  // columns that a CTA writes (rows of A, or outputs), four at a time, or gates and ups of eight; the last CTAs maybe fewer, or none
+  constexpr int UNIT = LANES_A && GATED ? 16 : 4;
+  const int own = columns_owned(NX, UNIT, p.split);
   if (warp < ADDERS) {
     if (!GROUPED) pdl_wait();
     const int row = 32 * (warp % 4) + lane, col0 = S::COLS * (warp / 4);
@@ -211,22 +232,33 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     float sum[S::COLS];
 #pragma unroll
     for (int j = 0; j < S::COLS; ++j) sum[j] = 0.f;
-    constexpr int PER = CHUNK * NX / (ADDERS * 32);
+    constexpr int PER = LANES_A ? 4 : CHUNK * NX / (ADDERS * 32);        // LANES_A: the scales of the next four blocks
     float next_a[PER], next_w[PER], next_up[PER];
     auto ask = [&](int first) {                          // the scales of a chunk that the thread brings, all at once
 #pragma unroll
       for (int x = 0; x < PER; ++x) {
-        const int at = threadIdx.x + x * ADDERS * 32, b = min(first + at / NX, nkb - 1), t = m0 + at % NX;
+        const int at = threadIdx.x + x * ADDERS * 32, b = min(first + (LANES_A ? x : at / NX), nkb - 1), t = m0 + (LANES_A ? row : at % NX);
         next_a[x] = t < p.M ? p.sa[(kb0 + b) * p.lds + t] : 0.f;
         next_w[x] = sw[b];
         next_up[x] = GATED ? sw[(long long)p.nb * p.blocks + b] : 0.f;
       }
     };
     if (nkb > 0) ask(0);
+    float four[PER] = {}, four_up[PER] = {};
     bool ok = true;                                      // once a wait gave up nothing is waited for any more (the warps still meet at their barriers)
     for (int i = 0; i < nkb; ++i) {
       const int h = i % S::NACC;
-      if (i % CHUNK == 0) {                              // this chunk's scales are in registers: to shared memory, and the next chunk's asked for
+      float f_row = 0.f, f_up = 0.f;
+      if (LANES_A) {                                     // the scales of the thread's row and of the tile's columns
+        if (i % PER == 0) {
+#pragma unroll
+          for (int x = 0; x < PER; ++x) four[x] = next_a[x] * next_w[x], four_up[x] = next_a[x] * next_up[x];
+          if (i + PER < nkb) ask(i + PER);
+        }
+        f_row = four[0], f_up = four_up[0];
+#pragma unroll
+        for (int x = 1; x < PER; ++x) four[x - 1] = four[x], four_up[x - 1] = four_up[x];
+      } else if (i % CHUNK == 0) {                       // this chunk's scales are in registers: to shared memory, and the next chunk's asked for
         if (i) asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
 #pragma unroll
         for (int x = 0; x < PER; ++x) {
@@ -237,7 +269,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (i + CHUNK < nkb) ask(i + CHUNK);
       }
       if (ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (i / S::NACC) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * (i % S::STAGES), (i / S::STAGES) & 1));
         if (!ok && lane == 0) atomicExch(p.status, ST_ADDER_TIMEOUT);
       }
       if (!ok) continue;
@@ -252,7 +284,8 @@ uint32_t x[PIECES][PIECE];
 #pragma unroll
       for (int c = 0; c < S::COLS; c += 4) {
         const uint32_t *v = &x[c / PIECE][c % PIECE];
-        const float4 s = *reinterpret_cast<const float4 *>(f + c);
+        const float g = GATED && (c & 8) ? f_up : f_row;
+        const float4 s = LANES_A ? make_float4(g, g, g, g) : *reinterpret_cast<const float4 *>(f + c);
         const float2 u0 = fma2(make_float2(__uint_as_float(v[0]), __uint_as_float(v[1])), make_float2(s.x, s.y), make_float2(sum[c], sum[c + 1]));
         const float2 u1 = fma2(make_float2(__uint_as_float(v[2]), __uint_as_float(v[3])), make_float2(s.z, s.w), make_float2(sum[c + 2], sum[c + 3]));
         sum[c] = u0.x, sum[c + 1] = u0.y, sum[c + 2] = u1.x, sum[c + 3] = u1.y;
@@ -264,13 +297,13 @@ uint32_t x[PIECES][PIECE];
     if (p.split == 1) {
 #pragma unroll
       for (int j = 0; j < S::COLS; j += 4)
-        sent[(col0 + j) / 4 * WM + row] = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
+        sent[(col0 + j) / 4 * S::PITCH + row] = make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]);
     } else {
       const uint32_t base = smem_addr(sent);
       int to = col0 / own, left = own - col0 % own;      // the owner of the columns at hand, and how many of its own are still to come
 #pragma unroll
       for (int j = 0; j < S::COLS; j += 4) {
-        const uint32_t at = base + ((rank * own + own - left) / 4 * WM + row) * 16;
+        const uint32_t at = base + ((rank * own + own - left) / 4 * S::PITCH + row) * 16;
         st_cluster(map_to_cta(at, (uint32_t)to), make_float4(sum[j], sum[j + 1], sum[j + 2], sum[j + 3]));
         left -= 4;
         if (left == 0) ++to, left = own;
@@ -286,29 +319,66 @@ uint32_t x[PIECES][PIECE];
     tc_fence_after();
     tmem_dealloc(tmem, S::TMEM);
   }
-  if (warp < ADDERS) {
+  // four columns from the `c`-th owned on, of lane r: the ranges' parts in their order
+  auto whole = [&](int c, int r) {
+    float4 v = sent[c / 4 * S::PITCH + r];
+#pragma unroll
+    for (int s = 1; s < MOST_SPLIT; ++s) {
+      if (s >= p.split) break;
+      const float4 x = sent[(s * own + c) / 4 * S::PITCH + r];
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+    }
+    return v;
+  };
+  if (warp < ADDERS && LANES_A) {                        // neighbouring lanes neighbouring fours of a row's outputs
+    constexpr int STEP = GATED ? 8 : 4;                  // columns behind four outputs
+    const int columns = min(own, NX - rank * own), fours = max(1, columns / STEP), n_out = GATED ? p.N / 2 : p.N;
+    const int first = (n0 + rank * own) / (GATED ? 2 : 1);
+    const bool vector = p.ldo % 4 == 0 && ((uintptr_t)p.out & (EPI == EPI_BF16 ? 7 : 15)) == 0;
+    for (int x = threadIdx.x; columns > 0 && x < LANES * fours; x += ADDERS * 32) {
+      const int r = x / fours, q = x - r * fours, n = first + 4 * q;
+      if (m0 + r >= end) break;
+      if (n >= n_out) continue;
+      const long long at = (long long)(m0 + r) * p.ldo + n;
+      float *const to = static_cast<float *>(p.out) + at;
+      const bool all = vector && n + 4 <= n_out;
+      float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (EPI == EPI_ADD_F32 && all) old = *reinterpret_cast<const float4 *>(to);
+      float4 v = whole(GATED ? (q >> 1) * 16 + (q & 1) * 4 : 4 * q, r);
+      if (GATED) {
+        const float4 u = whole((q >> 1) * 16 + (q & 1) * 4 + 8, r);
+        v = make_float4(glu_value(v.x, u.x, p.form), glu_value(v.y, u.y, p.form), glu_value(v.z, u.z, p.form), glu_value(v.w, u.w, p.form));
+      }
+      if (all) {
+        if (EPI == EPI_BF16) {
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+          *reinterpret_cast<uint2 *>(static_cast<bf16 *>(p.out) + at) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+        } else {
+          *reinterpret_cast<float4 *>(to) = EPI == EPI_ADD_F32 ? make_float4(old.x + v.x, old.y + v.y, old.z + v.z, old.w + v.w) : v;
+        }
+      } else {
+        const float vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (n + i >= n_out) break;
+          if (EPI == EPI_BF16) static_cast<bf16 *>(p.out)[at + i] = __float2bfloat16_rn(vs[i]);
+          else to[i] = EPI == EPI_ADD_F32 ? to[i] + vs[i] : vs[i];
+        }
+      }
+    }
+  } else if (warp < ADDERS) {                            // neighbouring lanes neighbouring outputs, four rows at a time
     const int t0 = m0 + rank * own, rows = min(min(own, NX - rank * own), end - t0);
-    constexpr int OUTS = GATED ? WM / 2 : WM;            // outputs of a row of A
+    constexpr int OUTS = GATED ? LANES / 2 : LANES;      // outputs of a row of A
     const int n = (GATED ? n0 / 2 : n0) + threadIdx.x % OUTS, n_out = GATED ? p.N / 2 : p.N;
     if (n < n_out) {
       const int l = threadIdx.x % OUTS, r0 = GATED ? (l >> 3) * 16 + (l & 7) : l;
-      const float4 *from = sent + r0;
       for (int c = threadIdx.x / OUTS * 4; c < rows; c += ADDERS * 32 / OUTS * 4) {
         const long long at = (long long)(t0 + c) * p.ldo + n;
-        float4 v = from[c / 4 * WM], u = GATED ? from[c / 4 * WM + 8] : v, old;
         float *const add = static_cast<float *>(p.out) + at;
+        float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
         if (EPI == EPI_ADD_F32)
           old = make_float4(add[0], c + 1 < rows ? add[p.ldo] : 0.f, c + 2 < rows ? add[2 * p.ldo] : 0.f, c + 3 < rows ? add[3 * p.ldo] : 0.f);
-#pragma unroll
-        for (int s = 1; s < 8; ++s) {
-          if (s >= p.split) break;
-          const float4 x = from[(s * own + c) / 4 * WM];
-          v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-          if (GATED) {
-            const float4 y = from[(s * own + c) / 4 * WM + 8];
-            u.x += y.x, u.y += y.y, u.z += y.z, u.w += y.w;
-          }
-        }
+        const float4 v = whole(c, r0), u = GATED ? whole(c, r0 + 8) : v;
         const float vs[4] = {v.x, v.y, v.z, v.w}, us[4] = {u.x, u.y, u.z, u.w}, olds[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -322,68 +392,70 @@ uint32_t x[PIECES][PIECE];
   }
 }
 
-template <int NX, int EPI, bool GROUPED>
+template <int NX, bool LANES_A, int EPI, bool GROUPED>
 static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
   static G2bPerDevice configured;
   const int dev = g2b_current_device();
   if (dev < 0 || !configured.value[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX>::SMEM);
-    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX>::SMEM, cudaGetErrorString(e));
+    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX, LANES_A>::SMEM);
+    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A>::SMEM, cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  const long long tiles_m = ((long long)p.M + NX - 1) / NX + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
-  const long long tiles_n = (p.N + WM - 1) / WM;
-  if (tiles_m > 65535 || tiles_n * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
-  g2b_launch_cluster(gemm_fp8_few_kernel<NX, EPI, GROUPED>, dim3((unsigned)(tiles_n * p.split), (unsigned)tiles_m), dim3(Shape<NX>::THREADS),
-                     (size_t)Shape<NX>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
+  const long long tiles_m = ((long long)p.M + Shape<NX, LANES_A>::ROWS_A - 1) / Shape<NX, LANES_A>::ROWS_A + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
+  const long long tiles_n = (p.N + Shape<NX, LANES_A>::ROWS_W - 1) / Shape<NX, LANES_A>::ROWS_W;
+  if (tiles_n > 65535 || tiles_m * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
+  g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED>, dim3((unsigned)(tiles_m * p.split), (unsigned)tiles_n), dim3(Shape<NX, LANES_A>::THREADS),
+                     (size_t)Shape<NX, LANES_A>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
   return g2b_check_launch("gemm_fp8_few");
 }
 
-template <int NX>
+template <int NX, bool LANES_A>
 static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
   if (p.starts) {
     switch (epi) {
-      case EPI_F32: return launch<NX, EPI_F32, true>(map_a, map_w, p, stream);
-      case EPI_GATED_F32: return launch<NX, EPI_GATED_F32, true>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<NX, LANES_A, EPI_F32, true>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, true>(map_a, map_w, p, stream);
     }
   } else {
     switch (epi) {
-      case EPI_BF16: return launch<NX, EPI_BF16, false>(map_a, map_w, p, stream);
-      case EPI_F32: return launch<NX, EPI_F32, false>(map_a, map_w, p, stream);
-      case EPI_ADD_F32: return launch<NX, EPI_ADD_F32, false>(map_a, map_w, p, stream);
-      case EPI_GATED_F32: return launch<NX, EPI_GATED_F32, false>(map_a, map_w, p, stream);
+      case EPI_BF16: return launch<NX, LANES_A, EPI_BF16, false>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<NX, LANES_A, EPI_F32, false>(map_a, map_w, p, stream);
+      case EPI_ADD_F32: return launch<NX, LANES_A, EPI_ADD_F32, false>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, false>(map_a, map_w, p, stream);
     }
   }
   G2B_REFUSE("gemm_fp8_few: no epilogue %d%s", epi, p.starts ? " for experts" : "");
 }
 
 // a [M, lda], w [N, ldw] (`starts`: [n_experts, N, ldw]), scales sa [blocks, lds] and sw [ceil(N / 128), blocks] (gated: [2, ceil(N / 256), blocks]; a
-// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side; split: parts of K, at
-// most 8.
+// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side, or,
+// `lanes_a`, 128 rows of w beside 128 of a; split: parts of K, at most 8.
 extern "C" int g2b_gemm_fp8_few(const void *a, const float *sa, const void *w, const float *sw, void *out, int M, int N, int blocks, long long lda,
                                 long long lds, long long ldw, long long ldo, int epi, float limit, float offset, float c1, float c3, const int *starts,
-                                int n_experts, int columns, int split, int *status, cudaStream_t stream) {
+                                int n_experts, int columns, int lanes_a, int split, int *status, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || blocks <= 0) return 0;
   if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_few: rows must start on 16 bytes");
   if (epi == EPI_GATED_F32 && N % 16) G2B_REFUSE("gemm_fp8_few: gates and ups in eights, got %d rows", N);
-  if (split < 1 || split > 8) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
+  if (split < 1 || split > MOST_SPLIT) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
   if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_few: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
   const long long w_rows = (long long)N * (starts ? n_experts : 1);
   if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %lld rows of W are too many", w_rows);
   CUtensorMap map_a, map_w;
-  int rc = columns > 0 && columns <= 256 ? get_map(&map_a, a, M, blocks * BK, (int)lda, columns, 1) : -1;
-  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, WM, 1);
+  int rc = columns > 0 && columns <= 256 ? get_map(&map_a, a, M, blocks * BK, (int)lda, lanes_a ? LANES : columns, 1) : -1;
+  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, lanes_a ? columns : LANES, 1);
   if (rc) G2B_REFUSE("gemm_fp8_few: cuTensorMapEncodeTiled failed (%d)", rc);
   Few p;
   p.sa = sa, p.sw = sw, p.out = out, p.starts = starts, p.status = status;
   p.M = M, p.N = N, p.blocks = blocks, p.n_experts = n_experts, p.nb = ((epi == EPI_GATED_F32 ? N / 2 : N) + F8_BLOCK - 1) / F8_BLOCK, p.split = split;
   p.lds = lds, p.ldo = ldo;
   p.form.limit = limit, p.form.offset = offset, p.form.c1 = c1, p.form.c3 = c3;
-  switch (columns) {
-    case 16: return pick<16>(epi, map_a, map_w, p, stream);
-    case 32: return pick<32>(epi, map_a, map_w, p, stream);
-    case 64: return pick<64>(epi, map_a, map_w, p, stream);
-    case 128: return pick<128>(epi, map_a, map_w, p, stream);
+  switch (lanes_a ? -columns : columns) {
+    case 16: return pick<16, false>(epi, map_a, map_w, p, stream);
+    case 32: return pick<32, false>(epi, map_a, map_w, p, stream);
+    case 64: return pick<64, false>(epi, map_a, map_w, p, stream);
+    case 128: return pick<128, false>(epi, map_a, map_w, p, stream);
+    case -128: return pick<128, true>(epi, map_a, map_w, p, stream);
+    case -64: return pick<64, true>(epi, map_a, map_w, p, stream);
   }
-  G2B_REFUSE("gemm_fp8_few: %d columns", columns);
+  G2B_REFUSE("gemm_fp8_few: no tiles of %d columns", columns);
 }

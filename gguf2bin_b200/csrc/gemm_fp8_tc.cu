@@ -33,7 +33,7 @@ constexpr int ADDERS = 8, THREADS = (ADDERS + 4) * 32;   // the last two warps o
 // Registers: 384 threads start with 168 each (64,512); the adders hold 128 sums and two pieces of an accumulator and take 232, the others
 // keep 40: 256 * 232 + 128 * 40 = 64,512.
 constexpr int ADDER_REGS = 232, OTHER_REGS = 40;
-constexpr int COLS = BN / 2, AT_ONCE = 32;
+constexpr int COLS = BN / 2, PIECE = 16;
 constexpr int RING_BYTES = STAGES * STAGE_BYTES;
 constexpr int MOST_EXPERTS = 1024;
 constexpr int BOX_BYTES = 32 * 128;                      // an adder's outputs on their way to C: 32 rows of 128 bytes, swizzled as the ring is
@@ -70,9 +70,8 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
 }
 // Waits for this thread's loads of tensor memory; the registers pass through, so that nothing that reads them moves in front.
 #define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
-__device__ __forceinline__ void loaded64(uint32_t (&a)[32], uint32_t (&b)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(a, 0), F8_RW8(a, 8), F8_RW8(a, 16), F8_RW8(a, 24) : : "memory");
-  asm volatile("" : F8_RW8(b, 0), F8_RW8(b, 8), F8_RW8(b, 16), F8_RW8(b, 24));
+__device__ __forceinline__ void loaded32(uint32_t (&a)[16], uint32_t (&b)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(a, 0), F8_RW8(a, 8), F8_RW8(b, 0), F8_RW8(b, 8) : : "memory");
 }
 // One arrival on a barrier of the pair: this warp's reads of tensor memory are done (they are waited for); it hands over no data.
 __device__ __forceinline__ void arrive_read(uint32_t cluster_bar) {
@@ -113,20 +112,19 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int OUT_BYTES = ADDERS * BOXES<GROUPED> * BOX_BYTES;
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + RING_BYTES + OUT_BYTES);
-  const uint32_t full0 = smem_addr(bars), empty0 = full0 + 8 * STAGES, sum_full0 = empty0 + 8 * STAGES, sum_empty0 = sum_full0 + 16;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 4);
+  // a stage's `done` says both that its operands are free and that its sums are there (so there are at least as many stages as accumulators: an
+  // adder has seen it before the stage's next products are issued).  A commit costs the tensor cores about 200 cycles: one a block, not two.
+  const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * STAGES, sum_empty0 = done0 + 8 * STAGES;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2);
   int *list = reinterpret_cast<int *>(smem + RING_BYTES + OUT_BYTES + BAR_BYTES);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t half = cluster_ctarank();               // the pair's first CTA issues its products
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full0 + 8 * s, 1);                       // in the first CTA, with both CTAs' bytes
-      mbar_init(empty0 + 8 * s, 1);
+      mbar_init(done0 + 8 * s, 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(sum_full0 + 8 * b, 1);
-      mbar_init(sum_empty0 + 8 * b, 2 * ADDERS);         // in the first CTA: both CTAs' adders
-    }
+    for (int b = 0; b < 2; ++b) mbar_init(sum_empty0 + 8 * b, 2 * ADDERS);      // in the first CTA: both CTAs' adders
     mbar_init_fence();
   }
   if (warp == ADDERS + 1) tmem_alloc_pair(smem_addr(tmem_slot), 2 * BN);
@@ -159,7 +157,8 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 
   if (warp >= ADDERS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(OTHER_REGS));
-    if (warp == ADDERS && lane == 0 && PRODUCER_RUNS) {
+    // Both loops are walked by their whole warps, with one lane elected around what is issued: see elect_one.
+    if (warp == ADDERS && PRODUCER_RUNS) {
       const uint32_t first_full0 = map_to_cta(full0, 0);
       bool ok = true;
       int it = 0;
@@ -168,39 +167,44 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const int row_a = tile.m0 + (int)half * BM, row_w = tile.e * p.N + tile.n0 + (int)half * BM;
         for (int b = 0; b < p.blocks; ++b, ++it) {
           const int s = it % STAGES;
-          if (it >= STAGES && !mbar_wait(empty0 + 8 * s, (it / STAGES - 1) & 1)) {
-            atomicExch(p.status, ST_PRODUCER_TIMEOUT);
-            ok = false;
+          if (it >= STAGES) ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * s, (it / STAGES - 1) & 1));
+          if (!ok) {
+            if (lane == 0) atomicExch(p.status, ST_PRODUCER_TIMEOUT);
             break;
           }
           const uint32_t to = smem_addr(smem + s * STAGE_BYTES);
-          if (half == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
-          tma_load_2d_pair(to, &map_a, b * BK, row_a, first_full0 + 8 * s);
-          tma_load_2d_pair(to + PART_BYTES, &map_w, b * BK, row_w, first_full0 + 8 * s);
+          if (elect_one()) {
+            if (half == 0) mbar_expect_tx(full0 + 8 * s, 2 * STAGE_BYTES);
+            tma_load_2d_pair(to, &map_a, b * BK, row_a, first_full0 + 8 * s);
+            tma_load_2d_pair(to + PART_BYTES, &map_w, b * BK, row_w, first_full0 + 8 * s);
+          }
+          __syncwarp();
         }
       }
     }
-    if (warp == ADDERS + 1 && lane == 0 && half == 0) {
+    if (warp == ADDERS + 1 && half == 0) {
       bool ok = true;
       int it = 0;
       for (int t = pair; t < n_tiles && ok; t += pairs)
         for (int b = 0; b < p.blocks; ++b, ++it) {
           const int s = it % STAGES, h = it & 1;
-          if (!mbar_wait(full0 + 8 * s, (it / STAGES) & 1) || (it >= 2 && !mbar_wait(sum_empty0 + 8 * h, (it / 2 - 1) & 1))) {
-            atomicExch(p.status, ST_MMA_TIMEOUT);
-            ok = false;
+          ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * s, (it / STAGES) & 1) && (it < 2 || mbar_wait(sum_empty0 + 8 * h, (it / 2 - 1) & 1)));
+          if (!ok) {
+            if (lane == 0) atomicExch(p.status, ST_MMA_TIMEOUT);
             break;
           }
           tc_fence_after();
           const uint32_t lo = ((smem_addr(smem + s * STAGE_BYTES) & 0x3FFFF) >> 4) | 1u << 16;
           const uint32_t to = tmem + h * BN;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (k == 0) umma_f8_pair<false>(to, lo, lo + PART_BYTES / 16, IDESC);
-            else umma_f8_pair<true>(to, lo + 2 * k, lo + PART_BYTES / 16 + 2 * k, IDESC);
+            for (int k = 0; k < 4; ++k) {
+              if (k == 0) umma_f8_pair<false>(to, lo, lo + PART_BYTES / 16, IDESC);
+              else umma_f8_pair<true>(to, lo + 2 * k, lo + PART_BYTES / 16 + 2 * k, IDESC);
+            }
+            umma_commit_pair(done0 + 8 * s, 3);
           }
-          umma_commit_pair(empty0 + 8 * s, 3);
-          umma_commit_pair(sum_full0 + 8 * h, 3);
+          __syncwarp();
         }
     }
     __syncwarp();
@@ -214,8 +218,8 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     bool ok = true;                                      // once a wait gave up nothing is waited for any more, and (but with EPI_GATED_ROWS, whose warps
     int it = 0;                                          // meet in pairs at every tile) nothing is written
     for (int t = pair; t < n_tiles; t += pairs) {
-      // Inside the loop over K the sums and the pieces of an accumulator take 192 of the 232 registers, so little else lives there: the tile is
-      // found again behind it, and the scales' places are 32-bit offsets (84 bytes of spills in this loop cost 401 -> 586 us).
+      // Inside the loop over K the sums and the pieces of an accumulator take 160 of the 232 registers and addresses most of
+      // the rest: the tile is found again behind it, and the scales' places are 32-bit offsets.
       int at_a, at_w;
       {
         const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
@@ -238,36 +242,38 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           if (GATED) next_up = p.sw[at_w + p.nb * p.blocks];
         }
         if (!ok) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(sum_full0 + 8 * h, (it / 2) & 1));      // the warp's lanes agree: its loads are all lanes'
+        ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * (it % STAGES), (it / STAGES) & 1));      // the warp's lanes agree: its loads are all lanes'
         if (!ok) {
           if (lane == 0) atomicExch(p.status, ST_ADDER_TIMEOUT);
           continue;
         }
         tc_fence_after();
-        // Two pieces of 32 columns are asked for at once, and the next two as the first ones are used: two waits a block.
-        uint32_t x[2][AT_ONCE];
-        const uint32_t from = from0 + h * BN;
-        auto add = [&](int c, const uint32_t (&v)[AT_ONCE]) {
+        // Two pieces of 16 columns are on their way while two are added.  (Of 32 columns the loop kept sums in memory: 380 -> 560 us.)
+        uint32_t x[2][PIECE];
+        auto add = [&](int c, const uint32_t (&v)[PIECE]) {
 #pragma unroll
-          for (int j = 0; j < AT_ONCE; j += 2) {
+          for (int j = 0; j < PIECE; j += 2) {
             const float fj = GATED && (j & 8) ? f_up : f;
             const float2 s = fma2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), make_float2(fj, fj), make_float2(sum[c + j], sum[c + j + 1]));
             sum[c + j] = s.x, sum[c + j + 1] = s.y;
           }
         };
-        tmem_ld32(from, x[0]);
-        tmem_ld32(from + 32, x[1]);
-        loaded64(x[0], x[1]);
-        add(0, x[0]);
-        tmem_ld32(from + 64, x[0]);
-        add(32, x[1]);
-        tmem_ld32(from + 96, x[1]);
-        loaded64(x[0], x[1]);
-        tc_fence_before();                               // the accumulator is read: its next products need not wait for these sums
-        __syncwarp();
-        if (lane == 0) arrive_read(first_empty0 + 8 * h);
-        add(64, x[0]);
-        add(96, x[1]);
+        const uint32_t from = from0 + h * BN;
+        tmem_ld16(from, x[0]);
+        tmem_ld16(from + 16, x[1]);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          loaded32(x[0], x[1]);
+          if (c + 32 == COLS) {                          // the accumulator is read: its next products need not wait for these sums
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_read(first_empty0 + 8 * h);
+          }
+          add(c, x[0]);
+          if (c + 32 < COLS) tmem_ld16(from + c + 32, x[0]);
+          add(c + 16, x[1]);
+          if (c + 32 < COLS) tmem_ld16(from + c + 48, x[1]);
+        }
       }
       if (!ok && EPI != EPI_GATED_ROWS) break;
       int again = t;

@@ -46,6 +46,13 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
+// One lane of a whole warp.  An issue loop that the warp walks together, with one lane elected around what it issues, keeps its addresses and
+// descriptors in uniform registers; a loop inside `if (lane == 0)` moves every one of them there for every instruction.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}\n" : "=r"(yes));
+  return yes != 0;
+}
 // true when the phase with the given parity has completed; false after SPIN_LIMIT polls
 // One probe first (test_wait: about 45 cycles on a B200), then try_wait, which may put the
 // thread to sleep but costs about 170 cycles even when the phase completed long ago.  More

@@ -168,15 +168,16 @@ def _product_tc(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, worksp
 
 
 def _product_few(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, columns: int, split: int, defines=()) -> None:
-    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile, K in ``split`` parts, at most 8."""
+    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile (-128: 128 on the lanes of tensor memory, beside 128 rows of the matrix),
+    K in ``split`` parts, at most 8."""
     if workspace is not None:
         workspace.waits = True
     f = _fn("gemm_fp8_few.cu", "g2b_gemm_fp8_few",
             [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int, *_FORM,
-             c_void_p, c_int, c_int, c_int, c_void_p, c_void_p], defines=tuple(defines))
+             c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p], defines=tuple(defines))
     _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(out), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
           rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], out.stride(0), epi, *form, _ptr(starts), w.q.shape[0] if starts is not None else 0,
-          columns, split, _ptr(_status_word(out.device)), _stream())
+          abs(columns), 1 if columns < 0 else 0, split, _ptr(_status_word(out.device)), _stream())
 
 
 MANY_ROWS = 128                      # rows (of an expert, on average) up to which a product goes to the kernel of few rows

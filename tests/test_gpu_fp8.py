@@ -390,7 +390,7 @@ def test_products_whose_copies_never_come(kernel):
     assert torch.equal(out, again) and out.abs().sum() > 0
 
 
-@pytest.mark.parametrize("columns", [16, 32, 64, 128])
+@pytest.mark.parametrize("columns", [16, 32, 64, 128, -128])
 @pytest.mark.parametrize("split", [1, 2, 3, 4, 7, 8])
 @pytest.mark.parametrize("M,N,K", [(1, 130, 300), (13, 128, 1024), (40, 300, 2176), (150, 200, 640), (5, 64, 5000)])
 def test_every_shape_of_few_rows(M, N, K, columns, split):
