@@ -1,13 +1,15 @@
 // Products in 8-bit floating point (fp8.cuh) of few rows, where the bytes of W are what counts:
 //   C[t, n] = sum_b s[b, t] S[n / 128, b] sum_{k in block b} q[t, k] Q[n, k].
 //
-// A CTA takes 128 rows of W (the M of a tcgen05.mma), NX rows of A (its N: 16, 32, 64 or 128) and a range of the blocks of K; the CTAs of a
+// A CTA takes 128 rows of W (the M of a tcgen05.mma), NX rows of A (its N: 16, 32 or 64) and a range of the blocks of K; the CTAs of a
 // cluster take the ranges of one tile.  A block's sums are formed in one of NACC accumulators in tensor memory.  Roles by warp:
 //   warps 0 .. 4 ADD - 1   add: a thread owns a row of W and 64 columns at most; it adds a finished accumulator, times the row's and the columns' scales
 //                          (their products are in shared memory, CHUNK blocks at a time), to its sums
 //   the next one           copies: STAGES blocks of W and A in flight.  W does not depend on what the stream ran before, so its first stages are
 //                          asked for before that has ended
-//   the last one           products
+//   the one behind it      products
+//   four more (FUSED)      quantise: up to 16 rows of activations come as they are (float32 or bfloat16); these warps quantise a block of them into
+//                          each stage as the copy of W comes in, and leave its scales for the adding warps
 // Behind its range every CTA sends its sums, column by column, to the CTA of the cluster that owns the column; that one adds them in the
 // order of the ranges and writes them, neighbouring lanes neighbouring outputs.  So a result depends on the sizes alone.
 //
@@ -15,19 +17,13 @@
 // ups of the same outputs, each with the scales of their own matrix.
 //
 // Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
-#include "fp8.cuh"
-#include "glu.cuh"
-#include "tc_common.cuh"
+#pragma once
+#include "product_fp8.cuh"
 
-G2B_DEFINE_LAST_ERROR
-
-using namespace tc;
-
-enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3 };
-enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
+namespace few {
 
 constexpr int LANES = 128, BK = F8_BLOCK, LANE_BYTES = LANES * BK;
-constexpr int MOST_EXPERTS = 1024;
+enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
 
 constexpr int MOST_SPLIT = 8;
 // columns that a CTA of `split` owns, `unit` at a time, and the most that ranges and columns owned come to
@@ -40,33 +36,28 @@ constexpr int most_sent(int columns, int unit) {
 }
 
 // LANES_A: the tile the other way round, 128 rows of A on the lanes of tensor memory and NX rows of W as its columns.
-// Two CTAs a multiprocessor (with 128 columns, one).
-template <int NX, bool LANES_A> struct Shape {
-  static constexpr int ADD = NX >= 64 ? 2 : 1;           // groups of four adding warps, 64 columns each at most
+// Two CTAs a multiprocessor.
+template <int NX, bool LANES_A, bool FUSED = false> struct Shape {
+  static constexpr int ADD = NX >= 64 ? 2 : 1;           // groups of four adding warps
   static constexpr int COLS = NX / ADD;
-  static constexpr int STAGES = NX == 16 ? 6 : NX == 32 ? 5 : NX == 64 ? 4 : 6;
+  static constexpr int STAGES = NX == 16 ? 6 : NX == 32 ? 5 : 4;
   static constexpr int NACC = 4;                         // at most STAGES: a stage's barrier says both that its operands and that its sums are done
   static constexpr int CHUNK = NX <= 32 ? 16 : 8;        // blocks whose scales are in shared memory at a time
   static constexpr int PITCH = LANES_A ? LANES + 1 : LANES;                           // of the columns sent: read along rows, or (LANES_A) along columns
   static constexpr int STAGE_BYTES = LANES * BK + NX * BK;
   static constexpr int RING = STAGES * STAGE_BYTES, SENT = most_sent(NX, LANES_A ? 16 : 4) / 4 * PITCH * 16;     // SENT lies where the ring was
   static constexpr int FACTORS = LANES_A ? 0 : 2 * CHUNK * NX * 4;
-  static constexpr int SMEM = RING + FACTORS + 256 + 1024;                            // + barriers, + the swizzle's alignment
-  static constexpr int THREADS = (4 * ADD + 2) * 32, PER_SM = NX == 128 ? 1 : 2;
+  static constexpr int SMEM = RING + FACTORS + 512 + 1024;                            // + barriers, + the swizzle's alignment
+  static constexpr int THREADS = (4 * ADD + 2 + (FUSED ? 4 : 0)) * 32, PER_SM = 2;
   static constexpr int TMEM = NACC * NX;
   static constexpr int ROWS_A = LANES_A ? LANES : NX, ROWS_W = LANES_A ? NX : LANES;
+  static_assert(!FUSED || (CHUNK > STAGES + NACC && NX == 16), "a block's scales stay until its sums are added");
   static_assert(NACC <= STAGES, "an adder must have seen a stage's barrier before its next products are issued");
   static_assert(SENT <= RING && PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * TMEM <= 512, "what a multiprocessor holds");
 };
 
-struct Few {
-  const float *sa, *sw;
-  void *out;
-  const int *starts;
-  int *status;
-  int M, N, blocks, n_experts, nb, split;                // nb: blocks of W's rows that have a scale
-  long long lds, ldo;
-  GluForm form;
+struct Few : Product {
+  int nb, split;                                         // nb: blocks of W's rows that have a scale
 };
 
 template <bool ACC>
@@ -85,7 +76,6 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float4 v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-#define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
 // Columns of this thread's lane: asked for, and waited for (the registers pass through the wait, so that nothing that reads them moves in front).
 __device__ __forceinline__ void ask_columns(uint32_t from, uint32_t (&x)[1][16]) { tmem_ld16(from, x[0]); }
 __device__ __forceinline__ void ask_columns(uint32_t from, uint32_t (&x)[1][32]) { tmem_ld32(from, x[0]); }
@@ -104,10 +94,10 @@ __device__ __forceinline__ void got_columns(uint32_t (&x)[2][32]) {
   asm volatile("" : F8_RW8(x[1], 0), F8_RW8(x[1], 8), F8_RW8(x[1], 16), F8_RW8(x[1], 24));
 }
 
-template <int NX, bool LANES_A, int EPI, bool GROUPED>
-__global__ void __launch_bounds__(Shape<NX, LANES_A>::THREADS, Shape<NX, LANES_A>::PER_SM)
+template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
+__global__ void __launch_bounds__(Shape<NX, LANES_A, FUSED>::THREADS, Shape<NX, LANES_A, FUSED>::PER_SM)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Few p) {
-  using S = Shape<NX, LANES_A>;
+  using S = Shape<NX, LANES_A, FUSED>;
   constexpr bool GATED = EPI == EPI_GATED_F32;
   constexpr int ADDERS = 4 * S::ADD, CHUNK = S::CHUNK, PIECE = S::COLS < 32 ? S::COLS : 32, PIECES = S::COLS / PIECE;
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(LANES >> 4) << 24);      // accumulator float, operands e4m3, K-major
@@ -117,8 +107,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   float4 *sent = reinterpret_cast<float4 *>(smem);                        // [range][four columns owned][row], behind the loop
   float *factors = reinterpret_cast<float *>(smem + S::RING);             // [gate, up][block of the chunk][column]
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::RING + S::FACTORS);
-  const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * S::STAGES, sum_empty0 = done0 + 8 * S::STAGES;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + S::NACC);
+  const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * S::STAGES, sum_empty0 = done0 + 8 * S::STAGES, scaled0 = sum_empty0 + 8 * S::NACC;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + S::NACC + (FUSED ? CHUNK : 0));
   int *found = reinterpret_cast<int *>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // (tiles of other rows of A, which read the same W, are neighbours)
@@ -126,10 +116,12 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   const int per = (p.blocks + p.split - 1) / p.split, kb0 = rank * per, nkb = max(0, min(p.blocks, kb0 + per) - kb0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(full0 + 8 * s, 1);
+      mbar_init(full0 + 8 * s, FUSED ? 5 : 1);           // the copies' bytes; the quantising warps
       mbar_init(done0 + 8 * s, 1);
     }
     for (int b = 0; b < S::NACC; ++b) mbar_init(sum_empty0 + 8 * b, ADDERS);
+    if (FUSED)
+      for (int b = 0; b < CHUNK; ++b) mbar_init(scaled0 + 8 * b, 4);
     mbar_init_fence();
   }
   int e = 0, m0 = tile_m * S::ROWS_A, end = p.M;
@@ -174,11 +166,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       const int ahead = min(nkb, S::STAGES);
       if (elect_one()) {
         for (int i = 0; i < ahead; ++i) {
-          mbar_expect_tx(full0 + 8 * i, S::STAGE_BYTES);
+          mbar_expect_tx(full0 + 8 * i, FUSED ? LANE_BYTES : S::STAGE_BYTES);
           tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_w, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * i);
         }
-        if (!GROUPED) pdl_wait();
-        for (int i = 0; i < ahead; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
+        if (!GROUPED && !FUSED) pdl_wait();
+        for (int i = 0; i < ahead && !FUSED; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
       }
       __syncwarp();
       for (int i = ahead; i < nkb; ++i) {
@@ -189,9 +181,9 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         }
         const uint32_t to = smem_addr(smem + s * S::STAGE_BYTES);
         if (elect_one()) {
-          mbar_expect_tx(full0 + 8 * s, S::STAGE_BYTES);
+          mbar_expect_tx(full0 + 8 * s, FUSED ? LANE_BYTES : S::STAGE_BYTES);
           tma_load_2d(to + at_w, &map_w, (kb0 + i) * BK, row_w, full0 + 8 * s);
-          tma_load_2d(to + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * s);
+          if (!FUSED) tma_load_2d(to + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * s);
         }
         __syncwarp();
       }
@@ -218,6 +210,78 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       }
       __syncwarp();
     }
+  } else if (FUSED && warp > ADDERS + 1) {
+    if (!GROUPED) pdl_wait();
+    // eight lanes a row, sixteen values each; AHEAD blocks are asked for before the first one is used
+    const int r = (threadIdx.x - (ADDERS + 2) * 32) / 8, part = threadIdx.x % 8;
+    const bool live = m0 + r < end;
+    const long long from = live ? (p.row_pair ? p.row_pair[m0 + r] / p.top : m0 + r) * p.x_stride : 0;
+    const int n_block = min((GATED ? n0 / 2 : n0) / F8_BLOCK, p.nb - 1);
+    const float *sw = p.sw + ((long long)e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks + kb0;
+    bool ok = true;
+    auto walk = [&](auto one) {
+      using T = decltype(one);
+      constexpr int PER16 = 16 / sizeof(T), LOADS = 16 / PER16, AHEAD = 8 / LOADS;
+      uint4 raw[AHEAD][LOADS];
+      float next_w[AHEAD], next_up[AHEAD];
+      auto ask = [&](int u, int i) {
+        if (i >= nkb) return;
+        const int k = (kb0 + i) * BK + 16 * part;        // K is a multiple of 8
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+          raw[u][j] = live && k + PER16 * j < p.K ? *reinterpret_cast<const uint4 *>(static_cast<const T *>(p.x) + from + k + PER16 * j) : make_uint4(0, 0, 0, 0);
+        next_w[u] = sw[i];
+        next_up[u] = GATED ? sw[(long long)p.nb * p.blocks + i] : 0.f;
+      };
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) ask(u, u);
+      for (int i0 = 0; i0 < nkb && ok; i0 += AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int i = i0 + u, s = i % S::STAGES;
+          if (i >= nkb || !ok) break;
+          float v[16], most = 0.f;
+#pragma unroll
+          for (int j = 0; j < LOADS; ++j) {
+            const uint32_t w[4] = {raw[u][j].x, raw[u][j].y, raw[u][j].z, raw[u][j].w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if constexpr (sizeof(T) == 4) v[4 * j + x] = __uint_as_float(w[x]);
+              else v[8 * j + 2 * x] = __uint_as_float(w[x] << 16), v[8 * j + 2 * x + 1] = __uint_as_float(w[x] & 0xffff0000u);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) most = max_nan(most, fabsf(v[j]));
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const BlockScale b = block_scale(most);
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = pack_e4m3(v[4 * j] * b.inverse, v[4 * j + 1] * b.inverse, v[4 * j + 2] * b.inverse, v[4 * j + 3] * b.inverse);
+          const float f = b.scale * next_w[u], f_up = b.scale * next_up[u];
+          ask(u, i + AHEAD);
+          if (i >= S::STAGES) ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * s, (i / S::STAGES - 1) & 1));
+          if (!ok) {
+            if (lane == 0) atomicExch(p.status, ST_PRODUCER_TIMEOUT);
+            break;
+          }
+          *reinterpret_cast<uint4 *>(smem + s * S::STAGE_BYTES + LANE_BYTES + r * 128 + ((part ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (part == 0) {
+            factors[i % CHUNK * NX + r] = f;
+            if (GATED) factors[CHUNK * NX + i % CHUNK * NX + r] = f_up;
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(full0 + 8 * s);
+            mbar_arrive(scaled0 + 8 * (i % CHUNK));
+          }
+        }
+      }
+    };
+    if (p.x_f32) walk(0.f);
+    else walk(bf16());
+    __syncwarp();
   }
   // columns that a CTA writes (rows of A, or outputs), four at a time, or gates and ups of eight; the last CTAs maybe fewer, or none
   constexpr int UNIT = LANES_A && GATED ? 16 : 4;
@@ -232,7 +296,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     float sum[S::COLS];
 #pragma unroll
     for (int j = 0; j < S::COLS; ++j) sum[j] = 0.f;
-    constexpr int PER = LANES_A ? 4 : CHUNK * NX / (ADDERS * 32);        // LANES_A: the scales of the next four blocks
+    constexpr int PER = FUSED ? 1 : LANES_A ? 4 : CHUNK * NX / (ADDERS * 32);        // LANES_A: the scales of the next four blocks
     float next_a[PER], next_w[PER], next_up[PER];
     auto ask = [&](int first) {                          // the scales of a chunk that the thread brings, all at once
 #pragma unroll
@@ -243,7 +307,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         next_up[x] = GATED ? sw[(long long)p.nb * p.blocks + b] : 0.f;
       }
     };
-    if (nkb > 0) ask(0);
+    if (nkb > 0 && !FUSED) ask(0);
     float four[PER] = {}, four_up[PER] = {};
     bool ok = true;                                      // once a wait gave up nothing is waited for any more (the warps still meet at their barriers)
     for (int i = 0; i < nkb; ++i) {
@@ -258,7 +322,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         f_row = four[0], f_up = four_up[0];
 #pragma unroll
         for (int x = 1; x < PER; ++x) four[x - 1] = four[x], four_up[x - 1] = four_up[x];
-      } else if (i % CHUNK == 0) {                       // this chunk's scales are in registers: to shared memory, and the next chunk's asked for
+      } else if (!FUSED && i % CHUNK == 0) {             // this chunk's scales are in registers: to shared memory, and the next chunk's asked for
         if (i) asm volatile("bar.sync 1, %0;\n" ::"n"(ADDERS * 32) : "memory");
 #pragma unroll
         for (int x = 0; x < PER; ++x) {
@@ -269,7 +333,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         if (i + CHUNK < nkb) ask(i + CHUNK);
       }
       if (ok) {
-        ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * (i % S::STAGES), (i / S::STAGES) & 1));
+        ok = __all_sync(0xffffffffu, (!FUSED || mbar_wait(scaled0 + 8 * (i % CHUNK), (i / CHUNK) & 1)) && mbar_wait(done0 + 8 * (i % S::STAGES), (i / S::STAGES) & 1));
         if (!ok && lane == 0) atomicExch(p.status, ST_ADDER_TIMEOUT);
       }
       if (!ok) continue;
@@ -392,70 +456,89 @@ uint32_t x[PIECES][PIECE];
   }
 }
 
-template <int NX, bool LANES_A, int EPI, bool GROUPED>
+template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
+static cudaError_t allow() {
+  return cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX, LANES_A, FUSED>::SMEM);
+}
+
+// How many CTAs in clusters of `split` the device holds at once.
+template <int NX, bool LANES_A, bool FUSED>
+static int resident(int split) {
+  static G2bPerDevice kept[MOST_SPLIT + 1];
+  const int dev = g2b_current_device();
+  if (dev >= 0 && kept[split].value[dev] > 0) return kept[split].value[dev];
+  int clusters = 0;
+  if (allow<NX, LANES_A, EPI_F32, false, FUSED>() == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(split), cfg.blockDim = dim3(Shape<NX, LANES_A, FUSED>::THREADS), cfg.dynamicSmemBytes = Shape<NX, LANES_A, FUSED>::SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = split, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&clusters, gemm_fp8_few_kernel<NX, LANES_A, EPI_F32, false, FUSED>, &cfg) != cudaSuccess) clusters = 0;
+  }
+  const int n = clusters > 0 ? clusters * split : 1;
+  if (dev >= 0) kept[split].value[dev] = n;
+  return n;
+}
+
+template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
 static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
   static G2bPerDevice configured;
   const int dev = g2b_current_device();
   if (dev < 0 || !configured.value[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX, LANES_A>::SMEM);
-    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A>::SMEM, cudaGetErrorString(e));
+    const cudaError_t e = allow<NX, LANES_A, EPI, GROUPED, FUSED>();
+    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A, FUSED>::SMEM, cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  const long long tiles_m = ((long long)p.M + Shape<NX, LANES_A>::ROWS_A - 1) / Shape<NX, LANES_A>::ROWS_A + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
-  const long long tiles_n = (p.N + Shape<NX, LANES_A>::ROWS_W - 1) / Shape<NX, LANES_A>::ROWS_W;
+  const long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED>::ROWS_A + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
+  const long long tiles_n = (p.N + Shape<NX, LANES_A, FUSED>::ROWS_W - 1) / Shape<NX, LANES_A, FUSED>::ROWS_W;
   if (tiles_n > 65535 || tiles_m * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
-  g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED>, dim3((unsigned)(tiles_m * p.split), (unsigned)tiles_n), dim3(Shape<NX, LANES_A>::THREADS),
-                     (size_t)Shape<NX, LANES_A>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
+  g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, dim3((unsigned)(tiles_m * p.split), (unsigned)tiles_n), dim3(Shape<NX, LANES_A, FUSED>::THREADS),
+                     (size_t)Shape<NX, LANES_A, FUSED>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
   return g2b_check_launch("gemm_fp8_few");
 }
 
-template <int NX, bool LANES_A>
+template <int NX, bool LANES_A, bool FUSED>
 static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
   if (p.starts) {
     switch (epi) {
-      case EPI_F32: return launch<NX, LANES_A, EPI_F32, true>(map_a, map_w, p, stream);
-      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, true>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<NX, LANES_A, EPI_F32, true, FUSED>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, true, FUSED>(map_a, map_w, p, stream);
     }
   } else {
     switch (epi) {
-      case EPI_BF16: return launch<NX, LANES_A, EPI_BF16, false>(map_a, map_w, p, stream);
-      case EPI_F32: return launch<NX, LANES_A, EPI_F32, false>(map_a, map_w, p, stream);
-      case EPI_ADD_F32: return launch<NX, LANES_A, EPI_ADD_F32, false>(map_a, map_w, p, stream);
-      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, false>(map_a, map_w, p, stream);
+      case EPI_BF16: return launch<NX, LANES_A, EPI_BF16, false, FUSED>(map_a, map_w, p, stream);
+      case EPI_F32: return launch<NX, LANES_A, EPI_F32, false, FUSED>(map_a, map_w, p, stream);
+      case EPI_ADD_F32: return launch<NX, LANES_A, EPI_ADD_F32, false, FUSED>(map_a, map_w, p, stream);
+      case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, false, FUSED>(map_a, map_w, p, stream);
     }
   }
   G2B_REFUSE("gemm_fp8_few: no epilogue %d%s", epi, p.starts ? " for experts" : "");
 }
 
-// a [M, lda], w [N, ldw] (`starts`: [n_experts, N, ldw]), scales sa [blocks, lds] and sw [ceil(N / 128), blocks] (gated: [2, ceil(N / 256), blocks]; a
-// stack: for every expert).  Rows of a and w on 16 bytes, zeros behind K.  columns: 16, 32, 64 or 128 rows of a side by side, or,
-// `lanes_a`, 128 rows of w beside 128 of a; split: parts of K, at most 8.
-extern "C" int g2b_gemm_fp8_few(const void *a, const float *sa, const void *w, const float *sw, void *out, int M, int N, int blocks, long long lda,
-                                long long lds, long long ldw, long long ldo, int epi, float limit, float offset, float c1, float c3, const int *starts,
-                                int n_experts, int columns, int lanes_a, int split, int *status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || blocks <= 0) return 0;
-  if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_few: rows must start on 16 bytes");
-  if (epi == EPI_GATED_F32 && N % 16) G2B_REFUSE("gemm_fp8_few: gates and ups in eights, got %d rows", N);
+// columns: 16, 32 or 64 rows of a side by side, or -64: 64 rows of w beside 128 of a; split: parts of K, at most 8.  With p.x (columns is 16 then): K a
+// multiple of 8 and every row of x on 16 bytes.
+static int run(const Product &given, int columns, int split, cudaStream_t stream) {
+  if (given.x && (columns != 16 || given.K % 8 || given.x_stride % (given.x_f32 ? 4 : 8) || ((uintptr_t)given.x & 15) || given.top < 1))
+    G2B_REFUSE("gemm_fp8_few: rows of %d values are not quantised on the way", given.K);
   if (split < 1 || split > MOST_SPLIT) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
-  if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_few: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
-  const long long w_rows = (long long)N * (starts ? n_experts : 1);
-  if (w_rows > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %lld rows of W are too many", w_rows);
   CUtensorMap map_a, map_w;
-  int rc = columns > 0 && columns <= 256 ? get_map(&map_a, a, M, blocks * BK, (int)lda, lanes_a ? LANES : columns, 1) : -1;
-  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, lanes_a ? columns : LANES, 1);
+  int rc = get_map(&map_w, given.w, given.w_rows(), given.blocks * BK, (int)given.ldw, columns < 0 ? 64 : LANES, 1);
+  if (given.x) map_a = map_w;
+  else if (!rc) rc = get_map(&map_a, given.a, given.M, given.blocks * BK, (int)given.lda, columns < 0 ? LANES : columns, 1);
   if (rc) G2B_REFUSE("gemm_fp8_few: cuTensorMapEncodeTiled failed (%d)", rc);
   Few p;
-  p.sa = sa, p.sw = sw, p.out = out, p.starts = starts, p.status = status;
-  p.M = M, p.N = N, p.blocks = blocks, p.n_experts = n_experts, p.nb = ((epi == EPI_GATED_F32 ? N / 2 : N) + F8_BLOCK - 1) / F8_BLOCK, p.split = split;
-  p.lds = lds, p.ldo = ldo;
-  p.form.limit = limit, p.form.offset = offset, p.form.c1 = c1, p.form.c3 = c3;
-  switch (lanes_a ? -columns : columns) {
-    case 16: return pick<16, false>(epi, map_a, map_w, p, stream);
-    case 32: return pick<32, false>(epi, map_a, map_w, p, stream);
-    case 64: return pick<64, false>(epi, map_a, map_w, p, stream);
-    case 128: return pick<128, false>(epi, map_a, map_w, p, stream);
-    case -128: return pick<128, true>(epi, map_a, map_w, p, stream);
-    case -64: return pick<64, true>(epi, map_a, map_w, p, stream);
+  static_cast<Product &>(p) = given;
+  p.nb = given.scale_rows(), p.split = split;
+  if (given.x) return pick<16, false, true>(given.epi, map_a, map_w, p, stream);
+  switch (columns) {
+    case 16: return pick<16, false, false>(given.epi, map_a, map_w, p, stream);
+    case 32: return pick<32, false, false>(given.epi, map_a, map_w, p, stream);
+    case 64: return pick<64, false, false>(given.epi, map_a, map_w, p, stream);
+    case -64: return pick<64, true, false>(given.epi, map_a, map_w, p, stream);
   }
   G2B_REFUSE("gemm_fp8_few: no tiles of %d columns", columns);
 }
+
+}  // namespace few

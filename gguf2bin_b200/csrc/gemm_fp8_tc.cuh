@@ -15,15 +15,11 @@
 // reads, so their scale is known where they are made.
 //
 // Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
-#include "fp8.cuh"
-#include "glu.cuh"
-#include "tc_common.cuh"
+#pragma once
+#include "product_fp8.cuh"
 
-G2B_DEFINE_LAST_ERROR
+namespace many {
 
-using namespace tc;
-
-enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3, EPI_GATED_ROWS = 4 };
 enum { ST_PRODUCER_TIMEOUT = 31, ST_MMA_TIMEOUT = 32, ST_ADDER_TIMEOUT = 33 };
 
 constexpr int BM = 128, BN = 256, BK = F8_BLOCK;        // BM: rows of a CTA
@@ -35,7 +31,6 @@ constexpr int ADDERS = 8, THREADS = (ADDERS + 4) * 32;   // the last two warps o
 constexpr int ADDER_REGS = 232, OTHER_REGS = 40;
 constexpr int COLS = BN / 2, PIECE = 16;
 constexpr int RING_BYTES = STAGES * STAGE_BYTES;
-constexpr int MOST_EXPERTS = 1024;
 constexpr int BOX_BYTES = 32 * 128;                      // an adder's outputs on their way to C: 32 rows of 128 bytes, swizzled as the ring is
 constexpr int BAR_BYTES = 256, LIST_BYTES = MOST_EXPERTS * 4;
 // Boxes of an adder: two where there is room, so that one is filled while the other is written out.
@@ -45,15 +40,8 @@ constexpr int SMEM = RING_BYTES + ADDERS * BOXES<GROUPED> * BOX_BYTES + BAR_BYTE
 static_assert(SMEM<false> <= 227 * 1024 && SMEM<true> <= 227 * 1024, "one CTA a multiprocessor");
 constexpr int BAND = 8;                                  // tiles along M that are walked side by side
 
-struct Tc {
-  const float *sa, *sw;
-  void *out;
-  float *out_scale;                                      // EPI_GATED_ROWS: [blocks of the outputs, ldos]
-  const int *starts;
-  int *status;
-  int M, N, blocks, n_experts, nb, boxes;                // nb: blocks of W's rows that have a scale; boxes: map_out may be used
-  long long lds, ldo, ldos;
-  GluForm form;
+struct Tc : Product {
+  int nb, boxes;                                         // nb: blocks of W's rows that have a scale; boxes: map_out may be used
 };
 
 template <bool ACC>
@@ -69,7 +57,6 @@ __device__ __forceinline__ void umma_f8_pair(uint32_t d, uint32_t a_lo, uint32_t
       : "memory");
 }
 // Waits for this thread's loads of tensor memory; the registers pass through, so that nothing that reads them moves in front.
-#define F8_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
 __device__ __forceinline__ void loaded32(uint32_t (&a)[16], uint32_t (&b)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" : F8_RW8(a, 0), F8_RW8(a, 8), F8_RW8(b, 0), F8_RW8(b, 8) : : "memory");
 }
@@ -433,34 +420,26 @@ static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, Tc p, cuda
   return g2b_check_launch("gemm_fp8_tc");
 }
 
-// As g2b_gemm_fp8_few (gemm_fp8_few.cu); with EPI_GATED_ROWS out is e4m3 [M, ldo] and out_scale float [ceil(N / 256), ldos].
-extern "C" int g2b_gemm_fp8_tc(const void *a, const float *sa, const void *w, const float *sw, void *out, float *out_scale, int M, int N, int blocks,
-                               long long lda, long long lds, long long ldw, long long ldo, long long ldos, int epi, float limit, float offset, float c1,
-                               float c3, const int *starts, int n_experts, int *status, cudaStream_t stream) {
-  if (M <= 0 || N <= 0 || blocks <= 0) return 0;
-  if (lda % 16 || ldw % 16 || (((uintptr_t)a | (uintptr_t)w) & 15)) G2B_REFUSE("gemm_fp8_tc: rows must start on 16 bytes");
-  const bool gated = epi >= EPI_GATED_F32;
-  if (gated && N % 16) G2B_REFUSE("gemm_fp8_tc: gates and ups in eights, got %d rows", N);
-  if (epi == EPI_GATED_ROWS && (ldo % 16 || ((uintptr_t)out & 15))) G2B_REFUSE("gemm_fp8_tc: quantised rows must start on 16 bytes");
-  if (starts && (n_experts < 1 || n_experts > MOST_EXPERTS)) G2B_REFUSE("gemm_fp8_tc: %d experts outside 1..%d", n_experts, MOST_EXPERTS);
-  const long long w_rows = (long long)N * (starts ? n_experts : 1);
-  if ((w_rows / F8_BLOCK + 2ll * n_experts + 2) * blocks > INT32_MAX || w_rows > INT32_MAX || lds * blocks > INT32_MAX || lda > INT32_MAX || ldw > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %d rows of A and %lld of W with %d blocks are too many for one launch", M, w_rows, blocks);
+static int resident() { return most_pairs<EPI_F32, false>() > 0 ? most_pairs<EPI_F32, false>() : 1; }
+
+static int run(const Product &given, cudaStream_t stream) {
+  const long long w_rows = given.w_rows();
+  if ((w_rows / F8_BLOCK + 2ll * given.n_experts + 2) * given.blocks > INT32_MAX || given.lds * given.blocks > INT32_MAX)
+    G2B_REFUSE("gemm_fp8_tc: %d rows of A and %lld of W with %d blocks are too many for one launch", given.M, w_rows, given.blocks);
   CUtensorMap map_a, map_w;
-  int rc = get_map(&map_a, a, M, blocks * BK, (int)lda, BM, 1);
-  if (!rc) rc = get_map(&map_w, w, w_rows, blocks * BK, (int)ldw, BM, 1);
+  int rc = get_map(&map_a, given.a, given.M, given.blocks * BK, (int)given.lda, BM, 1);
+  if (!rc) rc = get_map(&map_w, given.w, w_rows, given.blocks * BK, (int)given.ldw, BM, 1);
   if (rc) G2B_REFUSE("gemm_fp8_tc: cuTensorMapEncodeTiled failed (%d)", rc);
   Tc p;
-  p.sa = sa, p.sw = sw, p.out = out, p.out_scale = out_scale, p.starts = starts, p.status = status;
-  p.M = M, p.N = N, p.blocks = blocks, p.n_experts = n_experts, p.nb = ((gated ? N / 2 : N) + F8_BLOCK - 1) / F8_BLOCK;
-  p.lds = lds, p.ldo = ldo, p.ldos = ldos;
-  p.form.limit = limit, p.form.offset = offset, p.form.c1 = c1, p.form.c3 = c3;
-  if (starts) {
-    switch (epi) {
+  static_cast<Product &>(p) = given;
+  p.nb = given.scale_rows();
+  if (given.starts) {
+    switch (given.epi) {
       case EPI_F32: return launch<EPI_F32, true>(map_a, map_w, p, stream);
       case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, true>(map_a, map_w, p, stream);
     }
   } else {
-    switch (epi) {
+    switch (given.epi) {
       case EPI_BF16: return launch<EPI_BF16, false>(map_a, map_w, p, stream);
       case EPI_F32: return launch<EPI_F32, false>(map_a, map_w, p, stream);
       case EPI_ADD_F32: return launch<EPI_ADD_F32, false>(map_a, map_w, p, stream);
@@ -468,5 +447,7 @@ extern "C" int g2b_gemm_fp8_tc(const void *a, const float *sa, const void *w, co
       case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, false>(map_a, map_w, p, stream);
     }
   }
-  G2B_REFUSE("gemm_fp8_tc: no epilogue %d%s", epi, starts ? " for experts" : "");
+  G2B_REFUSE("gemm_fp8_tc: no epilogue %d%s", given.epi, given.starts ? " for experts" : "");
 }
+
+}  // namespace many

@@ -7,9 +7,8 @@
 //   moe_sort         the (token, choice) pairs in the order of their experts, stable: pairs of one expert keep their order, so a row's place depends on
 //                    the choices alone.  starts[e] .. starts[e + 1]: the rows of expert e.  Pairs of experts from `n_real` on get no row (-1).
 //   moe_back         y_t = sum_j weight_tj (row of pair (t, j), or the token's own input where the pair has none), in the order of j.
+#pragma once
 #include "fp8.cuh"
-
-G2B_DEFINE_LAST_ERROR
 
 // ---- rows -------------------------------------------------------------------------------------------------
 // Eight values of a row from column k on; zeros behind K.  VEC: every row on 16 bytes and K a multiple of 8.
@@ -87,7 +86,7 @@ static void launch_rows(bool vec, dim3 grid, cudaStream_t stream, const void *x,
 }
 
 // pair_row: int [tokens * top], or null (then every row of x has a row of q); places outside 0 .. n_rows - 1 are left out.  q's rows on 16 bytes.
-extern "C" int g2b_quantize_rows(const void *x, int dtype, long long x_stride, int tokens, int K, void *q, long long q_stride, float *scale,
+static int run_quantize_rows(const void *x, int dtype, long long x_stride, int tokens, int K, void *q, long long q_stride, float *scale,
                                  long long scale_stride, const int *pair_row, int top, int n_rows, cudaStream_t stream) {
   if (tokens <= 0 || K <= 0) return 0;
   const int blocks = (K + F8_BLOCK - 1) / F8_BLOCK;
@@ -143,7 +142,7 @@ quantize_matrix_kernel(const T *__restrict__ w, int N, int K, long long w_stride
 }
 
 // `count` matrices [N, K] one behind the other (`w_stride`, `q_stride`: from row to row); scale [count, ceil(N / 128), ceil(K / 128)].
-extern "C" int g2b_quantize_matrix(const void *w, int dtype, int count, int N, int K, long long w_stride, void *q, long long q_stride, float *scale,
+static int run_quantize_matrix(const void *w, int dtype, int count, int N, int K, long long w_stride, void *q, long long q_stride, float *scale,
                                    cudaStream_t stream) {
   if (count <= 0 || N <= 0 || K <= 0) return 0;
   const int kb = (K + F8_BLOCK - 1) / F8_BLOCK, nb = (N + F8_BLOCK - 1) / F8_BLOCK;
@@ -166,7 +165,7 @@ constexpr int SORT_WARPS = 32, SORT_MOST_EXPERTS = 1024;
 // One block.  A warp takes a stretch of the pairs, 32 at a time: lanes with one expert find each other (match), the first of them counts for
 // all.  No two warps share a counter, so nothing depends on who comes first.
 __global__ void __launch_bounds__(SORT_WARPS * 32)
-moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__restrict__ starts, int *__restrict__ pair_row) {
+moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__restrict__ starts, int *__restrict__ pair_row, int *__restrict__ row_pair) {
   extern __shared__ int at[];                    // [SORT_WARPS][n_real]: a warp's count of an expert, then the next row of its stretch
   __shared__ int warp_sum[SORT_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -221,15 +220,17 @@ moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__res
     const int p = p0 + lane, e = p < last ? idx[p] : -1;
     const uint32_t same = __match_any_sync(0xffffffffu, e);
     const bool real = e >= 0 && e < n_real;
-    if (p < last) pair_row[p] = real ? own[e] + __popc(same & ((1u << lane) - 1)) : -1;
+    const int row = real ? own[e] + __popc(same & ((1u << lane) - 1)) : -1;
+    if (p < last) pair_row[p] = row;
+    if (real && row_pair) row_pair[row] = p;
     __syncwarp();
     if (real && lane == __ffs(same) - 1) own[e] += __popc(same);
     __syncwarp();
   }
 }
 
-// starts: int [n_real + 1]
-extern "C" int g2b_moe_sort(const int *idx, int n_pairs, int n_real, int *starts, int *pair_row, cudaStream_t stream) {
+// starts: int [n_real + 1]; row_pair (the pair of every row in use) may be null
+static int run_moe_sort(const int *idx, int n_pairs, int n_real, int *starts, int *pair_row, int *row_pair, cudaStream_t stream) {
   if (n_real < 1 || n_real > SORT_MOST_EXPERTS) G2B_REFUSE("moe_sort: %d experts outside 1..%d", n_real, SORT_MOST_EXPERTS);
   static G2bPerDevice configured;
   const int dev = g2b_current_device();
@@ -238,7 +239,8 @@ extern "C" int g2b_moe_sort(const int *idx, int n_pairs, int n_real, int *starts
     if (e != cudaSuccess) G2B_REFUSE("moe_sort: %s", cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  g2b_launch(moe_sort_kernel, dim3(1), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * n_real * 4, stream, idx, max(n_pairs, 0), n_real, starts, pair_row);
+  g2b_launch(moe_sort_kernel, dim3(1), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * n_real * 4, stream, idx, max(n_pairs, 0), n_real, starts, pair_row,
+             row_pair);
   return g2b_check_launch("moe_sort");
 }
 
@@ -299,7 +301,7 @@ static void launch_back(int tokens, cudaStream_t stream, const float *rows, cons
 }
 
 // rows float [n_rows, H], x_self of `self_dtype`, out of `out_dtype`; everything on 16 bytes (bfloat16: 8), H and the strides multiples of 4.
-extern "C" int g2b_moe_back(const float *rows, const int *pair_row, const float *weight, const void *x_self, int self_dtype, long long self_stride,
+static int run_moe_back(const float *rows, const int *pair_row, const float *weight, const void *x_self, int self_dtype, long long self_stride,
                             int n_rows, int tokens, int top, int H, void *out, int out_dtype, long long out_stride, int accumulate, cudaStream_t stream) {
   if (tokens <= 0 || H <= 0) return 0;
   if (H % 4 || self_stride % 4 || out_stride % 4 || ((uintptr_t)rows & 15) || ((uintptr_t)x_self & (self_dtype == G2B_F32 ? 15 : 7)) ||

@@ -741,8 +741,8 @@ def gemm_f32_tc(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, accumulate:
 def linear(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor, accumulate: bool = False, workspace=None) -> None:
     """The product a layer asks for; picks the kernel from the dtypes and sizes.  Anything
     that is not all-bfloat16 runs on the float32 kernel (true 32-bit arithmetic), but for many rows in float32 with a
-    ``workspace`` for their parts (``gemm_f32_tc``).  With ``w`` in 8 bits (``Fp8Matrix``, ``Fp8Matrices``) ``a`` is quantised first (in the
-    workspace, or in new memory without one) unless it is ``Fp8Rows``; out is float32 or bfloat16."""
+    ``workspace`` for their parts (``gemm_f32_tc``).  With ``w`` in 8 bits (``Fp8Matrix``, ``Fp8Matrices``) ``a`` is quantised on the way, or
+    first (in the workspace, or in new memory without one), unless it is ``Fp8Rows``; out is float32 or bfloat16."""
     if isinstance(w, (Fp8Matrix, Fp8Matrices)):
         return (_fp8 or _fp8_mod()).linear(a, w, out, accumulate, workspace)
     if a.dtype == torch.bfloat16 and w.dtype == torch.bfloat16:

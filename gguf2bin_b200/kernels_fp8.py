@@ -1,7 +1,7 @@
 """Bindings of the kernels in 8-bit floating point (``csrc/fp8.cuh`` says how values are held)."""
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import Structure, addressof, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
@@ -14,7 +14,6 @@ BLOCK = 128                          # values of a row, and of either side of a 
 F8 = torch.float8_e4m3fn
 MOST_EXPERTS = 1024                  # csrc/quant_fp8.cu
 EPI_BF16, EPI_F32, EPI_ADD_F32, EPI_GATED_F32, EPI_GATED_ROWS = 0, 1, 2, 3, 4
-_FORM = [c_float] * 4
 
 
 def blocks_of(n: int) -> int:
@@ -30,12 +29,76 @@ def new_rows(tokens: int, k: int, workspace, name: str, device) -> Fp8Rows:
     return Fp8Rows(workspace.buffer(name + ".q", (tokens, kb * BLOCK), F8), workspace.buffer(name + ".scale", (kb, tokens), torch.float32))
 
 
+class _Call(Structure):
+    """What a call's sizes and types fix (csrc/products_fp8.cu)."""
+    _fields_ = [(n, c_longlong) for n in ("lda", "lds", "ldw", "ldo", "ldos", "x_stride")] + \
+        [(n, c_int) for n in ("M", "N", "K", "x_dtype", "epi", "n_experts", "top", "H", "columns", "split", "with_x", "columns_2", "split_2", "with_x_2")] + \
+        [(n, c_float) for n in ("limit", "offset", "c1", "c3")]
+
+
+class _Plan:
+    """A call that was checked once: every later one of the same sizes, strides, types, alignments and devices only passes its addresses."""
+    __slots__ = ("call", "at", "scratch", "status", "f")
+
+
+_plans: dict = {}
+BY_THE_RULE, WITH_X = 1, 17          # in place of columns 16, 32, 64, -64 (gemm_fp8_few.cuh) and 0 (gemm_fp8_tc.cuh); WITH_X: 16, quantised on the way
+
+
+def _f(name: str, argtypes, defines=()):
+    return _fn("products_fp8.cu", name, argtypes, defines=tuple(defines))
+
+
+def _plan(key, call: _Call, device, prepare: str, name: str, argtypes, x_aligned: bool, by_rule: bool = True, defines=()) -> _Plan:
+    plan = _Plan()
+    plan.call, plan.at = call, addressof(call)
+    size = _f(prepare, [c_void_p, c_int, c_int], defines)
+    size.restype = c_longlong
+    plan.scratch = size(plan.at, 1 if x_aligned else 0, 1 if by_rule else 0)
+    plan.status = _status_word(device).data_ptr()
+    plan.f = _f(name, argtypes, defines)
+    if len(_plans) > 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _launched(plan: _Plan, n: int) -> None:
+    """What a function of several launches returned: how many, or less than zero for an error."""
+    if n < 0:
+        raise KernelError(plan.f._lib.g2b_last_error().decode("utf-8", "replace"))
+    kernels.count_launches(n)
+
+
+def _scratch(plan: _Plan, workspace, name: str, device):
+    if workspace is not None:
+        workspace.waits = True
+        return workspace.buffer(name, (plan.scratch,), torch.uint8).data_ptr() if plan.scratch else None, None
+    if not plan.scratch:
+        return None, None
+    buf = torch.empty(plan.scratch, dtype=torch.uint8, device=device)
+    return buf.data_ptr(), buf
+
+
+def _here() -> int:
+    """The current device; -1 where there is none."""
+    try:
+        return torch.cuda.current_device() if kernels._raw_device is None else kernels._raw_device()
+    except RuntimeError:
+        return -1
+
+
+def _seen(t: torch.Tensor) -> tuple:
+    """What of a tensor a check may ask for."""
+    return t.shape, t.stride(), t.dtype, t.get_device(), t.data_ptr() & 15
+
+
 # ---- checks ----------------------------------------------------------------------------------------------------
 def _on_device(what: str, *tensors) -> None:
     at = [t.get_device() for t in tensors if t is not None]
     if min(at) < 0:
         raise KernelError(f"{what}: a tensor that is not on a CUDA device (there is no CPU path)")
-    here = torch.cuda.current_device() if kernels._raw_device is None else kernels._raw_device()
+    here = _here()
     if min(at) != here or max(at) != here:
         raise KernelError(f"{what}: tensors on the devices {sorted(set(at))}, while the current device is {here}")
 
@@ -65,21 +128,22 @@ def _check_matrix(what: str, w: Fp8Matrix, gated: bool, stacked: bool) -> None:
         raise KernelError(f"{what}: the matrix's scales are contiguous float32 {list(shape)}; got {s.dtype} {list(s.shape)}")
 
 
-def _quantised(what: str, a, k: int, workspace, name: str = "fp8.rows") -> Fp8Rows:
-    if isinstance(a, Fp8Rows):
-        _check_rows(what, a, k)
-        return a
-    if a.dim() != 2 or a.shape[1] != k:
-        raise KernelError(f"{what}: {list(a.shape)} values against a matrix of {k} columns")
-    rows = new_rows(a.shape[0], k, workspace, name, a.device)
-    quantize_rows(a, rows)
-    return rows
-
-
 # ---- rows and matrices -----------------------------------------------------------------------------------------
 def quantize_rows(x: torch.Tensor, rows: Fp8Rows, pair_row: Optional[torch.Tensor] = None) -> None:
     """``rows`` = x [T, K] (float32 or bfloat16) in 8 bits, a scale for every row and 128 columns; zeros behind K.
     ``pair_row`` int32 [T, top]: row t goes to the rows ``pair_row[t]`` instead (those below zero: nowhere)."""
+    q, scale = rows
+    key = (_seen(x), _seen(q), _seen(scale), None if pair_row is None else _seen(pair_row), _here())
+    plan = _plans.get(key) or _plan_rows(key, x, rows, pair_row)
+    f, given = plan
+    rc = f(x.data_ptr(), *given[0], q.data_ptr(), given[1], scale.data_ptr(), given[2], None if pair_row is None else pair_row.data_ptr(), given[3], given[4],
+           _stream())
+    if rc:
+        raise KernelError(f._lib.g2b_last_error().decode("utf-8", "replace"))
+    kernels.count_launches(1)
+
+
+def _plan_rows(key, x, rows: Fp8Rows, pair_row) -> tuple:
     if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         raise KernelError("quantize_rows: rows of neighbouring values")
     tokens, k = x.shape
@@ -94,12 +158,11 @@ def quantize_rows(x: torch.Tensor, rows: Fp8Rows, pair_row: Optional[torch.Tenso
     elif rows.q.shape[0] != tokens:
         raise KernelError(f"quantize_rows: {tokens} rows into {rows.q.shape[0]}")
     _on_device("quantize_rows", x, rows.q, rows.scale, pair_row)
-    if tokens == 0:
-        return
-    f = _fn("quant_fp8.cu", "g2b_quantize_rows", [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
-                                                  c_int, c_int, c_void_p])
-    _call(f, _ptr(x), _code(x.dtype), x.stride(0), tokens, k, _ptr(rows.q), rows.q.stride(0), _ptr(rows.scale), rows.scale.stride(0),
-          _ptr(pair_row), top, rows.q.shape[0], _stream())
+    f = _f("g2b_quantize_rows", [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p])
+    if len(_plans) > 4096:
+        _plans.clear()
+    plan = _plans[key] = (f, ((_code(x.dtype), x.stride(0), tokens, k), rows.q.stride(0), rows.scale.stride(0), top, rows.q.shape[0]))
+    return plan
 
 
 def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
@@ -111,7 +174,7 @@ def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
     lead = tuple(w.shape[:-2])
     q = torch.empty(lead + (n, blocks_of(k) * BLOCK), dtype=F8, device=w.device)
     scale = torch.empty(lead + (blocks_of(n), blocks_of(k)), dtype=torch.float32, device=w.device)
-    f = _fn("quant_fp8.cu", "g2b_quantize_matrix", [c_void_p, c_int, c_int, c_int, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p])
+    f = _f("g2b_quantize_matrix", [c_void_p, c_int, c_int, c_int, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p])
     _call(f, _ptr(w), _code(w.dtype), lead[0] if lead else 1, n, k, k, _ptr(q), q.shape[-1], _ptr(scale), _stream())
     return Fp8Matrix(q, scale, k)
 
@@ -153,120 +216,108 @@ def side_by_side(matrices):
 
 
 # ---- products --------------------------------------------------------------------------------------------------
-def _product_tc(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, defines=()) -> None:
-    """``out``: a tensor, or ``Fp8Rows`` with ``EPI_GATED_ROWS``."""
-    as_rows = epi == EPI_GATED_ROWS
-    to, scale = out if as_rows else (out, None)
-    if workspace is not None:
-        workspace.waits = True
-    f = _fn("gemm_fp8_tc.cu", "g2b_gemm_fp8_tc",
-            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong,
-             c_longlong, c_int, *_FORM, c_void_p, c_int, c_void_p, c_void_p], defines=tuple(defines))
-    _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(to), _ptr(scale), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
-          rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], to.stride(0), scale.stride(0) if as_rows else 0, epi, *form, _ptr(starts),
-          w.q.shape[0] if starts is not None else 0, _ptr(_status_word(to.device)), _stream())
-
-
-def _product_few(rows: Fp8Rows, w: Fp8Matrix, out, epi: int, form, starts, workspace, columns: int, split: int, defines=()) -> None:
-    """``columns`` (16, 32, 64 or 128) rows of activations side by side in a tile (-128: 128 on the lanes of tensor memory, beside 128 rows of the matrix),
-    K in ``split`` parts, at most 8."""
-    if workspace is not None:
-        workspace.waits = True
-    f = _fn("gemm_fp8_few.cu", "g2b_gemm_fp8_few",
-            [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_int, *_FORM,
-             c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p], defines=tuple(defines))
-    _call(f, _ptr(rows.q), _ptr(rows.scale), _ptr(w.q), _ptr(w.scale), _ptr(out), rows.q.shape[0], w.q.shape[-2], blocks_of(w.k),
-          rows.q.stride(0), rows.scale.stride(0), w.q.shape[-1], out.stride(0), epi, *form, _ptr(starts), w.q.shape[0] if starts is not None else 0,
-          abs(columns), 1 if columns < 0 else 0, split, _ptr(_status_word(out.device)), _stream())
-
-
-MANY_ROWS = 128                      # rows (of an expert, on average) up to which a product goes to the kernel of few rows
-
-
-def few_shape(rows: int, n: int, blocks: int, experts: int = 0) -> tuple:
-    """(columns, parts of K) of the kernel of few rows."""
-    each = -(-rows // experts) if experts else rows
-    columns = next((c for c in (16, 32, 64) if each <= c), 128)
-    tiles = -(-n // 128) * (min(experts, rows) if experts else -(-rows // columns))
-    most = 296 if columns <= 32 else 148           # CTAs that are there at once
-    split = 1
-    while split < 8 and tiles * split * 2 <= most and blocks >= 4 * split:
-        split *= 2
-    return columns, split
-
-
-def _product(rows: Fp8Rows, w: Fp8Matrix, out: torch.Tensor, epi: int, form=SILU, starts=None, workspace=None) -> None:
-    stacked, n = starts is not None, rows.q.shape[0]
-    if n > MANY_ROWS * (w.q.shape[0] if stacked else 1):
-        return _product_tc(rows, w, out, epi, form, starts, workspace)
-    if epi == EPI_GATED_ROWS:
-        inter = w.q.shape[-2] // 2
-        h = torch.empty((n, inter), dtype=torch.float32, device=w.q.device) if workspace is None else \
-            workspace.buffer("fp8.mid", (n, inter), torch.float32)
-        _product(rows, w, h, EPI_GATED_F32, form, starts, workspace)
-        return quantize_rows(h, out)
-    _product_few(rows, w, out, epi, form, starts, workspace, *few_shape(n, w.q.shape[-2], blocks_of(w.k), w.q.shape[0] if stacked else 0))
-
-
 def _check_out(what: str, out: torch.Tensor, rows: int, columns: int) -> None:
     if tuple(out.shape) != (rows, columns) or (columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns):
         raise KernelError(f"{what}: the output is [{rows}, {columns}], rows of neighbouring values that do not overlap; got {list(out.shape)} with "
                           f"strides {list(out.stride())}")
 
 
+def _check_values(what: str, a: torch.Tensor, k: int) -> None:
+    if a.dim() != 2 or a.shape[1] != k or a.dtype not in (torch.float32, torch.bfloat16) or (k > 1 and a.stride(1) != 1):
+        raise KernelError(f"{what}: {a.dtype} {list(a.shape)} with strides {list(a.stride())} against a matrix of {k} columns; rows of neighbouring "
+                          "float32 or bfloat16 values")
+
+
+def _plan_product(key, what: str, a, w: Fp8Matrix, out, epi: int, form, columns: int, split: int, defines) -> _Plan:
+    """Checks everything that a product's kernels rely on; ``epi`` below zero: whichever store the output's type asks for."""
+    gated = epi in (EPI_GATED_F32, EPI_GATED_ROWS)
+    as_rows, given = isinstance(out, Fp8Rows), isinstance(a, Fp8Rows)
+    _check_matrix(what, w, gated, False)
+    tokens = (a.q if given else a).shape[0]
+    n = w.q.shape[0] // 2 if gated else w.q.shape[0]
+    if as_rows:
+        _check_rows(what, out, n)
+        if out.q.shape[0] != tokens:
+            raise KernelError(f"{what}: {tokens} rows into {out.q.shape[0]}")
+    else:
+        _check_out(what, out, tokens, n)
+    if given:
+        _check_rows(what, a, w.k)
+    else:
+        _check_values(what, a, w.k)
+    _on_device(what, *(a if given else (a,)), w.q, w.scale, *(out if as_rows else (out,)))
+    call, to = _Call(), out.q if as_rows else out
+    call.M, call.N, call.K, call.epi = tokens, w.q.shape[0], w.k, epi
+    call.columns, call.split, call.with_x = 16 if columns == WITH_X else columns, split, 1 if columns == WITH_X else 0
+    call.ldw, call.ldo, call.ldos = w.q.shape[1], to.stride(0), out.scale.stride(0) if as_rows else 0
+    call.limit, call.offset, call.c1, call.c3 = form
+    if given:
+        call.x_dtype, call.lda, call.lds = -1, a.q.stride(0), a.scale.stride(0)
+    else:
+        call.x_dtype, call.x_stride = _code(a.dtype), a.stride(0)
+    return _plan(key, call, w.q.device, "g2b_fp8_product_plan", "g2b_fp8_product", [c_void_p] * 10, not given and a.data_ptr() % 16 == 0,
+                 columns == BY_THE_RULE, defines)
+
+
+def _product(what: str, a, w: Fp8Matrix, out, epi: int, form=SILU, workspace=None, columns: int = BY_THE_RULE, split: int = 1, defines=()) -> None:
+    """``columns`` and ``split``: the tiles of ``gemm_fp8_few.cuh`` and the parts of K (``BY_THE_RULE``: what ``choose`` in products_fp8.cu says)."""
+    q, s, k = w
+    given, as_rows = isinstance(a, Fp8Rows), isinstance(out, Fp8Rows)
+    key = (_seen(a.q) + _seen(a.scale) if given else _seen(a), _seen(q), _seen(s), k, _seen(out.q) + _seen(out.scale) if as_rows else _seen(out), epi, form,
+           _here(), columns, split, defines)
+    plan = _plans.get(key) or _plan_product(key, what, a, w, out, epi, form, columns, split, defines)
+    scratch, held = _scratch(plan, workspace, "fp8.product", q.device)
+    n = plan.f(plan.at, a.q.data_ptr() if given else a.data_ptr(), a.scale.data_ptr() if given else None, scratch, q.data_ptr(), s.data_ptr(),
+               out.q.data_ptr() if as_rows else out.data_ptr(), out.scale.data_ptr() if as_rows else None, plan.status, _stream())
+    _launched(plan, n)
+
+
 def linear(a, w, out: torch.Tensor, accumulate: bool, workspace) -> None:
     if isinstance(w, Fp8Matrices):
-        rows, at = _quantised("linear", a, w.parts[0].k, workspace), 0
-        _check_out("linear", out, rows.q.shape[0], w.shape[0])
+        rows, at = a, 0
+        _check_out("linear", out, (a.q if isinstance(a, Fp8Rows) else a).shape[0], w.shape[0])
+        if not isinstance(a, Fp8Rows):                   # quantised once for all of them
+            _check_values("linear", a, w.parts[0].k)
+            rows = new_rows(a.shape[0], w.parts[0].k, workspace, "fp8.rows", a.device)
+            quantize_rows(a, rows)
         for part in w.parts:
             n = part.q.shape[0]
             linear(rows, part, out[:, at:at + n], accumulate, workspace)
             at += n
         return
-    _check_matrix("linear", w, False, False)
-    tokens = a.q.shape[0] if isinstance(a, Fp8Rows) else a.shape[0]
-    _check_out("linear", out, tokens, w.q.shape[0])
-    if out.dtype not in (torch.float32, torch.bfloat16) or (accumulate and out.dtype != torch.float32):
+    if out.dtype == torch.float32:
+        epi = EPI_ADD_F32 if accumulate else EPI_F32
+    elif out.dtype == torch.bfloat16 and not accumulate:
+        epi = EPI_BF16
+    else:
         raise KernelError(f"linear: stores float32 or bfloat16 and adds to float32; got {out.dtype}")
-    rows = _quantised("linear", a, w.k, workspace)
-    _on_device("linear", rows.q, rows.scale, w.q, w.scale, out)
-    if tokens:
-        _product(rows, w, out, EPI_ADD_F32 if accumulate else EPI_F32 if out.dtype == torch.float32 else EPI_BF16, workspace=workspace)
+    _product("linear", a, w, out, epi, SILU, workspace)
 
 
 def gate_up(a, w: Fp8Matrix, mid, form, workspace) -> None:
     """mid = glu(gate, up) of a @ w.T, in float32 [T, I], or quantised (``Fp8Rows``)."""
-    _check_matrix("gate_up_fused", w, True, False)
-    tokens, inter = a.q.shape[0] if isinstance(a, Fp8Rows) else a.shape[0], w.q.shape[0] // 2
-    as_rows = isinstance(mid, Fp8Rows)
-    if as_rows:
-        _check_rows("gate_up_fused", mid, inter)
-        if mid.q.shape[0] != tokens:
-            raise KernelError(f"gate_up_fused: {tokens} rows into {mid.q.shape[0]}")
-    else:
-        _check_out("gate_up_fused", mid, tokens, inter)
-        if mid.dtype != torch.float32:
-            raise KernelError(f"gate_up_fused: a matrix in 8 bits leaves float32 or quantised rows, not {mid.dtype}")
-    rows = _quantised("gate_up_fused", a, w.k, workspace)
-    _on_device("gate_up_fused", rows.q, rows.scale, w.q, w.scale, mid.q if as_rows else mid)
-    if tokens:
-        _product(rows, w, mid, EPI_GATED_ROWS if as_rows else EPI_GATED_F32, form, workspace=workspace)
+    if isinstance(mid, Fp8Rows):
+        return _product("gate_up_fused", a, w, mid, EPI_GATED_ROWS, form, workspace)
+    if mid.dtype != torch.float32:
+        raise KernelError(f"gate_up_fused: a matrix in 8 bits leaves float32 or quantised rows, not {mid.dtype}")
+    _product("gate_up_fused", a, w, mid, EPI_GATED_F32, form, workspace)
 
 
 # ---- experts ---------------------------------------------------------------------------------------------------
-def moe_sort(idx: torch.Tensor, n_real: int, starts: torch.Tensor, pair_row: torch.Tensor) -> None:
+def moe_sort(idx: torch.Tensor, n_real: int, starts: torch.Tensor, pair_row: torch.Tensor, row_pair: Optional[torch.Tensor] = None) -> None:
     """Rows for the (token, choice) pairs of ``idx``, expert by expert and within an expert in their order: ``starts`` int32 [n_real + 1],
-    ``pair_row`` int32 like idx (-1: an expert from ``n_real`` on)."""
-    for t, what, n in ((idx, "idx", idx.numel()), (starts, "starts", n_real + 1), (pair_row, "pair_row", idx.numel())):
+    ``pair_row`` int32 like idx (-1: an expert from ``n_real`` on); ``row_pair``, where given: the pair of every row that one has."""
+    for t, what, n in ((idx, "idx", idx.numel()), (starts, "starts", n_real + 1), (pair_row, "pair_row", idx.numel()), (row_pair, "row_pair", idx.numel())):
+        if t is None:
+            continue
         if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
             raise KernelError(f"moe_sort: {what} is contiguous int32 of {n}; got {t.dtype} {list(t.shape)}")
-    _on_device("moe_sort", idx, starts, pair_row)
-    f = _fn("quant_fp8.cu", "g2b_moe_sort", [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p])
-    _call(f, _ptr(idx), idx.numel(), n_real, _ptr(starts), _ptr(pair_row), _stream())
+    _on_device("moe_sort", idx, starts, pair_row, row_pair)
+    f = _f("g2b_moe_sort", [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+    _call(f, _ptr(idx), idx.numel(), n_real, _ptr(starts), _ptr(pair_row), _ptr(row_pair), _stream())
 
 
-def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32: torch.Tensor, pair_row: torch.Tensor, form,
-                workspace) -> None:
+def _plan_experts(key, h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, pair_row, form) -> _Plan:
     what = "moe_experts_fp8"
     _check_matrix(what, w_gate_up, True, True)
     _check_matrix(what, w_down, False, True)
@@ -274,32 +325,49 @@ def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down
     if w_down.k != inter or w_down.q.shape[0] != n_experts:
         raise KernelError(f"{what}: gate and up of {n_experts} experts with {inter} outputs against down matrices {list(w_down.q.shape)} of "
                           f"{w_down.k} columns")
-    if h.dim() != 2 or idx.dim() != 2 or idx.shape[0] != h.shape[0] or h.shape[1] != w_gate_up.k:
-        raise KernelError(f"{what}: tokens {list(h.shape)} and choices {list(idx.shape)} for matrices of {w_gate_up.k} columns")
+    _check_values(what, h, w_gate_up.k)
+    if idx.dim() != 2 or idx.shape[0] != h.shape[0] or idx.dtype != torch.int32 or not idx.is_contiguous():
+        raise KernelError(f"{what}: choices are contiguous int32 [{h.shape[0]}, top]; got {idx.dtype} {list(idx.shape)}")
     if n_experts > MOST_EXPERTS:
         raise KernelError(f"{what}: {n_experts} experts, at most {MOST_EXPERTS}")
     n_pairs = idx.numel()
     if rows32.dtype != torch.float32 or tuple(rows32.shape) != (n_pairs, w_down.q.shape[1]) or not rows32.is_contiguous():
         raise KernelError(f"{what}: the experts' rows are contiguous float32 [{n_pairs}, {w_down.q.shape[1]}]")
+    if pair_row.dtype != torch.int32 or pair_row.numel() != n_pairs or not pair_row.is_contiguous():
+        raise KernelError(f"{what}: pair_row is contiguous int32 of {n_pairs}")
     _on_device(what, h, idx, w_gate_up.q, w_gate_up.scale, w_down.q, w_down.scale, rows32, pair_row)
-    if not n_pairs:
-        return
+    call = _Call()
+    call.M, call.N, call.K, call.x_dtype, call.n_experts = h.shape[0], 2 * inter, w_gate_up.k, _code(h.dtype), n_experts
+    call.top, call.H, call.x_stride, call.ldw = idx.shape[1], w_down.q.shape[1], h.stride(0), w_gate_up.q.shape[2]
+    call.limit, call.offset, call.c1, call.c3 = form
+    return _plan(key, call, h.device, "g2b_fp8_experts_plan", "g2b_fp8_experts", [c_void_p] * 12, h.data_ptr() % 16 == 0)
 
-    def scratch(name, shape, dtype):
-        return torch.empty(shape, dtype=dtype, device=h.device) if workspace is None else workspace.buffer(name, shape, dtype)
 
-    starts = scratch("fp8.starts", (n_experts + 1,), torch.int32)
-    moe_sort(idx, n_experts, starts, pair_row)
-    rows = new_rows(n_pairs, w_gate_up.k, workspace, "fp8.sorted", h.device)
-    quantize_rows(h, rows, pair_row)
-    mid = new_rows(n_pairs, inter, workspace, "fp8.mid_rows", h.device)
-    _product(rows, w_gate_up, mid, EPI_GATED_ROWS, form, starts, workspace)
-    _product(mid, w_down, rows32, EPI_F32, SILU, starts, workspace)
+def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32: torch.Tensor, pair_row: torch.Tensor, form,
+                workspace) -> None:
+    gq, gs, gk = w_gate_up
+    dq, ds, dk = w_down
+    key = (_seen(h), _seen(idx), _seen(gq), _seen(gs), gk, _seen(dq), _seen(ds), dk, _seen(rows32), _seen(pair_row), form, _here())
+    plan = _plans.get(key) or _plan_experts(key, h, idx, w_gate_up, w_down, rows32, pair_row, form)
+    scratch, held = _scratch(plan, workspace, "fp8.experts", gq.device)
+    _launched(plan, plan.f(plan.at, h.data_ptr(), idx.data_ptr(), scratch, gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(), rows32.data_ptr(),
+                           pair_row.data_ptr(), plan.status, _stream()))
 
 
 def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool) -> None:
+    key = (_seen(rows32), _seen(pair_row), _seen(weight), _seen(x_self), _seen(out), accumulate, _here())
+    f, given = _plans.get(key) or _plan_back(key, rows32, pair_row, weight, x_self, out, accumulate)
+    rc = f(rows32.data_ptr(), pair_row.data_ptr(), weight.data_ptr(), x_self.data_ptr(), *given[0], out.data_ptr(), *given[1], _stream())
+    if rc:
+        raise KernelError(f._lib.g2b_last_error().decode("utf-8", "replace"))
+    kernels.count_launches(1)
+
+
+def _plan_back(key, rows32, pair_row, weight, x_self, out, accumulate: bool) -> tuple:
+    if weight.dim() != 2 or out.dim() != 2:
+        raise KernelError("moe_back: weights [tokens, top] and an output [tokens, width]")
     tokens, top = weight.shape
-    width = out.shape[-1]
+    width = out.shape[1]
     if weight.dtype != torch.float32 or not weight.is_contiguous() or pair_row.dtype != torch.int32 or not pair_row.is_contiguous() or \
             pair_row.numel() != tokens * top:
         raise KernelError(f"moe_back: weights are contiguous float32 [{tokens}, {top}], rows of the pairs as many int32")
@@ -310,7 +378,8 @@ def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool) -> None:
     if accumulate and out.dtype != torch.float32:
         raise KernelError("moe_back: only a float32 output is added to")
     _on_device("moe_back", rows32, pair_row, weight, x_self, out)
-    f = _fn("quant_fp8.cu", "g2b_moe_back", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p,
-                                             c_int, c_longlong, c_int, c_void_p])
-    _call(f, _ptr(rows32), _ptr(pair_row), _ptr(weight), _ptr(x_self), _code(x_self.dtype), x_self.stride(0), rows32.shape[0], tokens, top, width, _ptr(out),
-          _code(out.dtype), out.stride(0), 1 if accumulate else 0, _stream())
+    f = _f("g2b_moe_back", [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_void_p, c_int, c_longlong, c_int, c_void_p])
+    if len(_plans) > 4096:
+        _plans.clear()
+    plan = _plans[key] = (f, ((_code(x_self.dtype), x_self.stride(0), rows32.shape[0], tokens, top, width), (_code(out.dtype), out.stride(0), 1 if accumulate else 0)))
+    return plan
