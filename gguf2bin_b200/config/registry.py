@@ -10,6 +10,7 @@ import os
 from pathlib import Path
 from typing import Any, Callable, Mapping
 
+from .eight_bit import with_eight_bit
 from .specs import ConfigError, ModelSpec
 
 _ARCHITECTURES: dict[str, Callable[[Mapping[str, Any]], ModelSpec]] = {}
@@ -59,7 +60,7 @@ def model_spec_from_dict(d: Mapping[str, Any]) -> ModelSpec:
     if name not in _ARCHITECTURES:
         raise ConfigError(f"config.json: architecture {name!r} is not registered; registered: "
                           + ", ".join(registered_architectures()))
-    return _ARCHITECTURES[name](d)
+    return with_eight_bit(_ARCHITECTURES[name](d), d)
 
 
 def read_config_json(folder) -> dict:

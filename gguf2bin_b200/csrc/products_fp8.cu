@@ -30,12 +30,12 @@ struct Choice { int columns, split, with_x; };
 //   start + (parts + part * split, where K is in parts) + the 4-norm of (the rounds of CTAs: n blocks each, and `wave` for every round but one) and
 //   (W's bytes at `rate` TB/s);  a block takes `alone` where no two CTAs share a multiprocessor, else `block`.
 // Fitted to 2,200 times of 150 products (1 to 1,500 rows, 256 to 30,000 outputs, K = 512 to 17,408; graphs of products behind one another): within
-// 6 to 9 % (root mean square of the logarithm); what the estimates choose is 2 % slower than the best choice in the mean.  With the tiles the
+// 6 to 9 % (root mean square of the logarithm); what the estimates choose is 1 % slower than the best choice in the mean, 16 at worst.  With the tiles the
 // largest that fit instead, 64 rows by 5,120 x 17,408 took 34 us (21), and 128 rows by 6,144 x 4,096 13.9 (11.1).
 struct Cost { double start, parts, part, alone, block, wave, rate; };
-constexpr Cost COST_X = {2.05, 0.61, 0.10, 0.355, 0.405, 2.7, 5.9}, COST_16 = {2.00, 0.53, 0.09, 0.239, 0.350, 2.5, 6.6},
-               COST_32 = {2.50, 0.45, 0.12, 0.269, 0.422, 2.9, 6.6}, COST_64 = {2.59, 0.51, 0.22, 0.362, 0.576, 3.5, 5.2},
-               COST_LANES = {2.68, 0.15, 0.37, 0.272, 0.422, 3.4, 7.1};
+constexpr Cost COST_X = {2.11, 0.62, 0.09, 0.347, 0.345, 2.2, 5.8}, COST_16 = {2.02, 0.57, 0.08, 0.237, 0.320, 1.9, 6.5},
+               COST_32 = {2.50, 0.47, 0.10, 0.272, 0.421, 2.3, 6.8}, COST_64 = {2.60, 0.64, 0.19, 0.361, 0.558, 2.6, 5.2},
+               COST_LANES = {2.69, 0.28, 0.32, 0.276, 0.420, 2.8, 9.4};
 constexpr double QUANTISED_FIRST = 2.0;                  // a kernel of its own in front
 
 static double estimate(const Cost &k, long long tiles, int blocks, int split, int most, double w_bytes) {
@@ -47,26 +47,26 @@ static double estimate(const Cost &k, long long tiles, int blocks, int split, in
   return k.start + (split > 1 ? k.parts + k.part * split : 0) + __builtin_sqrt(__builtin_sqrt(w2 * w2 + b2 * b2));
 }
 
-// The cheapest.  `experts`: the rows are theirs, as many for each (those that have any), give or take.  with_x: the activations may be quantised on
-// the way; rows_needed: quantised rows are to be left (only gemm_fp8_tc.cuh leaves them itself).
-static Choice choose(int M, int N, int blocks, int experts, bool with_x, bool rows_needed) {
+// The cheapest for activations that are still to be quantised; given rows go the same way, so that they have the same bits.  `experts`: the rows are
+// theirs, as many for each (those that have any), give or take.  rows_needed: quantised rows are to be left (only gemm_fp8_tc.cuh leaves them itself).
+static Choice choose(int M, int N, int blocks, int experts, bool rows_needed) {
   const int used = experts ? (experts < M ? experts : M) : 1, each = (M + used - 1) / used;
   const double w_bytes = (double)used * N * blocks * F8_BLOCK;
   const double behind = rows_needed ? QUANTISED_FIRST + 1e-6 * M * N * 2.5 / 4 : 0;      // float, read and written again
   const long long pairs_tiles = (long long)used * ((each + 255) / 256) * ((N + 255) / 256);
   const int pairs = many::resident();
   Choice best = {0, 1, 0};
-  double least = QUANTISED_FIRST * with_x + 2.4 + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * 0.418 + 1.9);
+  double least = QUANTISED_FIRST + 2.4 + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * 0.418 + 1.9);
   auto look = [&](int columns, bool x, const Cost &k, int (*resident)(int)) {
     const int rows_a = columns > 0 ? columns : 128, rows_w = columns > 0 ? 128 : 64;
     const long long tiles = (long long)used * ((each + rows_a - 1) / rows_a) * ((N + rows_w - 1) / rows_w);
     if (tiles > INT32_MAX / few::MOST_SPLIT) return;
     for (int split = 1; split <= few::MOST_SPLIT && split <= blocks; ++split) {
-      const double us = estimate(k, tiles, blocks, split, resident(split), w_bytes) + (with_x && !x ? QUANTISED_FIRST : 0) + behind;
+      const double us = estimate(k, tiles, blocks, split, resident(split), w_bytes) + (x ? 0 : QUANTISED_FIRST) + behind;
       if (us < least) least = us, best = {columns, split, x};
     }
   };
-  if (each <= 16 && with_x) look(16, true, COST_X, few::resident<16, false, true>);
+  if (each <= 16) look(16, true, COST_X, few::resident<16, false, true>);
   if (each <= 48) look(16, false, COST_16, few::resident<16, false, false>);
   if (each > 8 && each <= 64) look(32, false, COST_32, few::resident<32, false, false>);
   if (each > 16 && each <= 128) look(64, false, COST_64, few::resident<64, false, false>);
@@ -128,7 +128,7 @@ static bool by_way_of_float(const Call &c) { return c.epi == EPI_GATED_ROWS && c
 // Chooses the kernel (by_rule: else c->first stands) and returns the bytes of scratch memory that the product takes; x_aligned: x starts on 16 bytes.
 extern "C" long long g2b_fp8_product_plan(Call *c, int x_aligned, int by_rule) {
   const bool with_x = may_be_on_the_way(*c, x_aligned != 0);
-  if (by_rule) c->first = choose(c->M, c->N, (c->K + F8_BLOCK - 1) / F8_BLOCK, 0, with_x, c->epi == EPI_GATED_ROWS);
+  if (by_rule) c->first = choose(c->M, c->N, (c->K + F8_BLOCK - 1) / F8_BLOCK, 0, c->epi == EPI_GATED_ROWS);
   if (!with_x) c->first.with_x = 0;
   size_t bytes = 0;
   if (c->x_dtype >= 0 && !c->first.with_x) bytes += rows_bytes(c->M, c->K);
@@ -172,12 +172,13 @@ extern "C" long long g2b_fp8_experts_plan(Call *c, int x_aligned, int by_rule) {
   size_t bytes = on_16((size_t)(c->n_experts + 1) * 4);
   if (pairs > INT32_MAX) return (long long)bytes;        // (the call refuses it)
   if (by_rule) {
-    c->first = choose((int)pairs, c->N, blocks, c->n_experts, may_be_on_the_way(*c, x_aligned != 0), false);
-    if (!c->first.with_x) c->first = choose((int)pairs, c->N, blocks, c->n_experts, false, true);
-    c->second = choose((int)pairs, c->H, blocks_down, c->n_experts, c->first.with_x != 0, false);
+    c->first = choose((int)pairs, c->N, blocks, c->n_experts, false);
+    if (!c->first.with_x) c->first = choose((int)pairs, c->N, blocks, c->n_experts, true);
+    c->second = choose((int)pairs, c->H, blocks_down, c->n_experts, false);
     if (!c->second.with_x) c->first.with_x = 0;          // both fetch their rows, or neither
   }
   if (!may_be_on_the_way(*c, x_aligned != 0)) c->first.with_x = 0;
+  if (!c->first.with_x) c->second.with_x = 0;
   if (c->first.with_x) return (long long)(bytes + on_16((size_t)pairs * 4) + on_16((size_t)pairs * inter * 4));
   bytes += rows_bytes(pairs, c->K) + rows_bytes(pairs, inter);
   if (c->first.columns) bytes += on_16((size_t)pairs * inter * 4);

@@ -10,24 +10,28 @@
 #pragma once
 #include "fp8.cuh"
 
+// ---- four values ---------------------------------------------------------------------------------------
+__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
+__device__ __forceinline__ float4 load4(const bf16 *p) {
+  const uint2 w = *reinterpret_cast<const uint2 *>(p);
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+}
+
 // ---- rows -------------------------------------------------------------------------------------------------
-// Eight values of a row from column k on; zeros behind K.  VEC: every row on 16 bytes and K a multiple of 8.
-template <typename T, bool VEC>
+// Eight values of a row from column k on; zeros behind K.  VEC = 8: every row on 16 bytes and K a multiple of 8; 4: the same of fours (bfloat16: on 8
+// bytes); 1: anything.
+template <typename T, int VEC>
 __device__ __forceinline__ void load8(const T *x, int k, int K, float (&v)[8]) {
-  if (VEC) {
-    if (k < K) {
-      if (sizeof(T) == 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(x + k), b = *reinterpret_cast<const float4 *>(x + k + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-      } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(x + k);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  if (VEC == 8 && sizeof(T) == 2) {
+    const uint4 a = k < K ? *reinterpret_cast<const uint4 *>(x + k) : make_uint4(0, 0, 0, 0);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    } else {
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  } else if (VEC >= 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    for (int h = 0; h < 8; h += 4) {
+      const float4 a = k + h < K ? load4(x + k + h) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[h] = a.x, v[h + 1] = a.y, v[h + 2] = a.z, v[h + 3] = a.w;
     }
   } else {
 #pragma unroll
@@ -38,7 +42,7 @@ __device__ __forceinline__ void load8(const T *x, int k, int K, float (&v)[8]) {
 constexpr int ROWS_AT_ONCE = 16, BLOCKS_AT_ONCE = 4;
 
 // Sixteen lanes a row, eight values each; a block of threads takes 16 rows x 4 blocks of 128.
-template <typename T, bool VEC>
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T *__restrict__ x, long long x_stride, int tokens, int K, int blocks, uint8_t *__restrict__ q, long long q_stride,
                      float *__restrict__ scale, long long scale_stride, const int *__restrict__ pair_row, int top, int n_rows) {
@@ -79,9 +83,9 @@ quantize_rows_kernel(const T *__restrict__ x, long long x_stride, int tokens, in
 }
 
 template <typename T>
-static void launch_rows(bool vec, dim3 grid, cudaStream_t stream, const void *x, long long x_stride, int tokens, int K, int blocks, void *q,
+static void launch_rows(int vec, dim3 grid, cudaStream_t stream, const void *x, long long x_stride, int tokens, int K, int blocks, void *q,
                         long long q_stride, float *scale, long long scale_stride, const int *pair_row, int top, int n_rows) {
-  g2b_launch(vec ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, grid, dim3(256), 0, stream, (const T *)x, x_stride, tokens, K,
+  g2b_launch(vec == 8 ? quantize_rows_kernel<T, 8> : vec == 4 ? quantize_rows_kernel<T, 4> : quantize_rows_kernel<T, 1>, grid, dim3(256), 0, stream, (const T *)x, x_stride, tokens, K,
              blocks, (uint8_t *)q, q_stride, scale, scale_stride, pair_row, top, n_rows);
 }
 
@@ -95,8 +99,8 @@ static int run_quantize_rows(const void *x, int dtype, long long x_stride, int t
   const int steps = (blocks + BLOCKS_AT_ONCE - 1) / BLOCKS_AT_ONCE;
   if (steps > 65535) G2B_REFUSE("quantize_rows: K=%d is too large", K);
   const dim3 grid((unsigned)((tokens + ROWS_AT_ONCE - 1) / ROWS_AT_ONCE), (unsigned)steps);
-  const int per16 = dtype == G2B_F32 ? 4 : 8;
-  const bool vec = K % 8 == 0 && x_stride % per16 == 0 && ((uintptr_t)x & 15) == 0;
+  const int whole = (K | (int)(x_stride & 7)) & 7, odd = (int)((uintptr_t)x & 15);
+  const int vec = whole == 0 && odd == 0 ? 8 : whole % 4 == 0 && (dtype == G2B_F32 ? odd == 0 : odd % 8 == 0) ? 4 : 1;
   if (dtype == G2B_F32)
     launch_rows<float>(vec, grid, stream, x, x_stride, tokens, K, blocks, q, q_stride, scale, scale_stride, pair_row, top, n_rows);
   else if (dtype == G2B_BF16)
@@ -160,13 +164,14 @@ static int run_quantize_matrix(const void *w, int dtype, int count, int N, int K
 }
 
 // ---- pairs by expert --------------------------------------------------------------------------------------
-constexpr int SORT_WARPS = 32, SORT_MOST_EXPERTS = 1024;
+constexpr int SORT_WARPS = 32, SORT_MOST_EXPERTS = 1024, SORT_AHEAD = 8;
 
-// One block.  A warp takes a stretch of the pairs, 32 at a time: lanes with one expert find each other (match), the first of them counts for
-// all.  No two warps share a counter, so nothing depends on who comes first.
+// One block.  A warp takes a stretch of the pairs, 32 at a time: lanes with one expert find each other (a ballot a bit of its number: match.any
+// takes 48 cycles of the multiprocessor, 27 us for 16,384 pairs; this 9), the first of them counts for all.  No two warps share a counter, so
+// nothing depends on who comes first.  A pair's place among its warp's waits in pair_row for the rows in front of it.
 __global__ void __launch_bounds__(SORT_WARPS * 32)
-moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__restrict__ starts, int *__restrict__ pair_row, int *__restrict__ row_pair) {
-  extern __shared__ int at[];                    // [SORT_WARPS][n_real]: a warp's count of an expert, then the next row of its stretch
+moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int bits, int *__restrict__ starts, int *pair_row, int *__restrict__ row_pair) {
+  extern __shared__ int at[];                    // [SORT_WARPS][n_real]: a warp's count of an expert, then the first row of its stretch
   __shared__ int warp_sum[SORT_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch();
@@ -176,11 +181,27 @@ moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__res
   pdl_wait();
   __syncthreads();
   int *own = at + warp * n_real;
-  for (int p0 = first; p0 < last; p0 += 32) {
-    const int p = p0 + lane, e = p < last ? idx[p] : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && e < n_real && lane == __ffs(same) - 1) own[e] += __popc(same);
-    __syncwarp();
+  for (int p0 = first; p0 < last; p0 += 32 * SORT_AHEAD) {
+    int e[SORT_AHEAD];
+#pragma unroll
+    for (int u = 0; u < SORT_AHEAD; ++u) e[u] = p0 + 32 * u + lane < last ? idx[p0 + 32 * u + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < SORT_AHEAD; ++u) {
+      const int p = p0 + 32 * u + lane;
+      if (p0 + 32 * u >= last) break;
+      const bool real = e[u] >= 0 && e[u] < n_real;
+      uint32_t same = __ballot_sync(0xffffffffu, real);
+      for (int b = 0; b < bits; ++b) {
+        const uint32_t set = __ballot_sync(0xffffffffu, e[u] >> b & 1);
+        same &= e[u] >> b & 1 ? set : ~set;
+      }
+      const uint32_t before = same & ((1u << lane) - 1);
+      const int count = real ? own[e[u]] : 0;
+      if (p < last) pair_row[p] = real ? count + __popc(before) : -1;
+      __syncwarp();
+      if (real && !before) own[e[u]] = count + __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   // rows of the experts before thread e's: a scan over the block, an expert a thread
@@ -216,16 +237,13 @@ moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int *__res
     }
   }
   __syncthreads();
-  for (int p0 = first; p0 < last; p0 += 32) {
-    const int p = p0 + lane, e = p < last ? idx[p] : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    const bool real = e >= 0 && e < n_real;
-    const int row = real ? own[e] + __popc(same & ((1u << lane) - 1)) : -1;
-    if (p < last) pair_row[p] = row;
-    if (real && row_pair) row_pair[row] = p;
-    __syncwarp();
-    if (real && lane == __ffs(same) - 1) own[e] += __popc(same);
-    __syncwarp();
+#pragma unroll 4
+  for (int p = first + lane; p < last; p += 32) {
+    const int rank = pair_row[p];
+    if (rank < 0) continue;
+    const int row = own[idx[p]] + rank;
+    pair_row[p] = row;
+    if (row_pair) row_pair[row] = p;
   }
 }
 
@@ -239,18 +257,12 @@ static int run_moe_sort(const int *idx, int n_pairs, int n_real, int *starts, in
     if (e != cudaSuccess) G2B_REFUSE("moe_sort: %s", cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  g2b_launch(moe_sort_kernel, dim3(1), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * n_real * 4, stream, idx, max(n_pairs, 0), n_real, starts, pair_row,
-             row_pair);
+  g2b_launch(moe_sort_kernel, dim3(1), dim3(SORT_WARPS * 32), (size_t)SORT_WARPS * n_real * 4, stream, idx, max(n_pairs, 0), n_real,
+             n_real > 1 ? 32 - __builtin_clz(n_real - 1) : 0, starts, pair_row, row_pair);
   return g2b_check_launch("moe_sort");
 }
 
 // ---- back to the tokens -----------------------------------------------------------------------------------
-__device__ __forceinline__ float4 load4(const float *p) { return *reinterpret_cast<const float4 *>(p); }
-__device__ __forceinline__ float4 load4(const bf16 *p) {
-  const uint2 w = *reinterpret_cast<const uint2 *>(p);
-  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-}
-
 // Four neighbours a thread; H a multiple of 4.
 template <typename TSELF, typename TOUT, bool ACCUM>
 __global__ void __launch_bounds__(256)

@@ -10,6 +10,7 @@ from . import kernels
 from .kernels_bf16 import _status_word
 from .kernels import SILU, Fp8Matrices, Fp8Matrix, Fp8Rows, KernelError, _call, _code, _fn, _ptr, _stream
 
+ON_THE_WAY = 16                      # rows up to which a product quantises them itself (csrc/products_fp8.cu, choose)
 BLOCK = 128                          # values of a row, and of either side of a matrix, that share a scale
 F8 = torch.float8_e4m3fn
 MOST_EXPERTS = 1024                  # csrc/quant_fp8.cu

@@ -11,14 +11,20 @@ limit), down( g sigmoid(alpha g) (u + 1) ), ``alpha`` 1.702 unless the spec says
 ``activation`` = "gelu_tanh": the gate's activation is the tanh form of GELU, 0.5 z (1 + tanh(sqrt(2/pi) (z +
 0.044715 z^3))), instead of SiLU.  All of these are one form with four numbers (``kernels.GluForm``), which the
 products' epilogues take.
+
+With ``eight_bit`` in its spec a part of the kinds ``swiglu`` and ``routed_experts`` has its matrices in 8-bit floating point, a scale for
+each 128 x 128, and quantises what they are multiplied with (``kernels.linear``, ``gate_up_fused``, ``moe_experts_fp8``); what lies between gate/up
+and down is quantised from 32 bits.
 """
 from __future__ import annotations
 
 import torch
 
-from .. import kernels
+from .. import kernels, kernels_fp8
 from ..config.specs import ConfigError, PartSpec
+from ..weights.eight_bit import expect_eight_bit
 from ..weights.loader import Expected
+from .eight_bit import flat_weights, held_tensors
 from .fused import normed_linear
 from .registry import feed_forward_class, register_feed_forward
 
@@ -43,6 +49,9 @@ class SwiGLU:
         self.block = 8 if self.inter % 8 == 0 else self.inter
         self.dtype = dtype
         self.names = dict(spec["names"])
+        self.eight_bit = bool(spec.get("eight_bit") or False)
+        if self.eight_bit and self.inter % 8:
+            raise ConfigError(f"swiglu: in 8 bits the width between is a multiple of 8, not {self.inter}")
         self.w_gate_up = self.w_down = None
         self.limit = float(spec.get("limit") or 0.0)
         self.alpha = float(spec.get("alpha") if spec.get("alpha") is not None else 1.702)
@@ -51,10 +60,16 @@ class SwiGLU:
     @classmethod
     def expected(cls, spec: PartSpec, hidden_size: int) -> dict:
         n, inter = dict(spec["names"]), spec["intermediate_size"]
-        return {n["gate"]: Expected((inter, hidden_size)), n["up"]: Expected((inter, hidden_size)),
-                n["down"]: Expected((hidden_size, inter))}
+        out = {n["gate"]: Expected((inter, hidden_size)), n["up"]: Expected((inter, hidden_size)),
+               n["down"]: Expected((hidden_size, inter))}
+        return expect_eight_bit(out, list(out)) if spec.get("eight_bit") else out
 
     def bind(self, tensors: dict) -> None:
+        if self.eight_bit:
+            tensors = held_tensors(tensors)
+            self.w_gate_up = kernels_fp8.gate_up_matrix(tensors[self.names["gate"]], tensors[self.names["up"]])
+            self.w_down = tensors[self.names["down"]]
+            return
         g, u = tensors[self.names["gate"]], tensors[self.names["up"]]
         if g.dtype != u.dtype:
             g, u = g.to(torch.float32), u.to(torch.float32)
@@ -65,7 +80,7 @@ class SwiGLU:
         self.w_down = tensors[self.names["down"]].contiguous()
 
     def weights(self):
-        return (self.w_gate_up, self.w_down)
+        return flat_weights(self.w_gate_up, self.w_down)
 
     def absorb_norm_weight(self, norm) -> bool:
         """As ``GQAAttention.absorb_norm_weight``, into the columns of the gate/up matrix."""
@@ -90,6 +105,13 @@ class SwiGLU:
     def _run(self, h, ctx, out32, accumulate: bool) -> None:
         T = h.shape[0]
         ws = ctx.workspace
+        if self.eight_bit:
+            # few rows stay in 32 bits, the down product quantises them itself; many are quantised where they are made
+            mid = ws.buffer("ffn.mid", (T, self.inter), torch.float32) if T <= kernels_fp8.ON_THE_WAY else \
+                kernels_fp8.new_rows(T, self.inter, ws, "ffn.mid", h.device)
+            kernels.gate_up_fused(h, self.w_gate_up, mid, self.block, self.form, ws)
+            kernels.linear(mid, self.w_down, out32, accumulate=accumulate, workspace=ws)
+            return
         mid = ws.buffer("ffn.mid", (T, self.inter), self.dtype)
         if not kernels.gate_up_fused(h, self.w_gate_up, mid, self.block, self.form):
             gu = ws.buffer("ffn.gate_up", (T, 2 * self.inter), self.dtype)
@@ -99,7 +121,7 @@ class SwiGLU:
 
     def forward_from_stream(self, x32: torch.Tensor, norm, ctx, residual32: torch.Tensor) -> None:
         """The same with the block's norm folded into the gate/up product."""
-        if self.form != kernels.SILU:  # the products that norm their own input know the plain SiLU gate only
+        if self.form != kernels.SILU or self.eight_bit:  # the products that norm their own input know the plain SiLU gate, and not 8 bits
             h = ctx.workspace.buffer("fused.normed", tuple(x32.shape), self.dtype)
             norm.forward(x32, h)
             return self.forward(h, ctx, residual32)
@@ -224,6 +246,9 @@ class RoutedExperts:
         if self.E < 0 or self.I < 0 or not (1 <= self.top <= self.E + self.I) or self.E > 1024:
             raise ConfigError(f"routed_experts: {self.top} choices among {self.E} + {self.I} experts")
         self.names = dict(spec["names"])
+        self.eight_bit = bool(spec.get("eight_bit") or False) and self.E > 0
+        if self.eight_bit and self.inter % 8:
+            raise ConfigError(f"routed_experts: in 8 bits the width between is a multiple of 8, not {self.inter}")
         self.w_router = self.correction = self.router_bias = self.w_gate_up = self.w_down = None
         self.has_bias = bool(spec.get("router_bias") or False)
         self.form = gate_form("routed_experts", None, float(spec.get("limit") or 0.0),
@@ -250,10 +275,12 @@ class RoutedExperts:
             out[n["correction"]] = Expected((E + I,))
         if spec.get("router_bias"):
             out[n["router_bias"]] = Expected((E + I,))
+        matrices = {}
         for e in range(E):
-            out[n["gate"].format(e)] = Expected((inter, hidden_size))
-            out[n["up"].format(e)] = Expected((inter, hidden_size))
-            out[n["down"].format(e)] = Expected((hidden_size, inter))
+            matrices[n["gate"].format(e)] = Expected((inter, hidden_size))
+            matrices[n["up"].format(e)] = Expected((inter, hidden_size))
+            matrices[n["down"].format(e)] = Expected((hidden_size, inter))
+        out.update(expect_eight_bit(matrices, list(matrices)) if spec.get("eight_bit") else matrices)
         if spec.get("shared") is not None:
             out.update(feed_forward_class(spec["shared"]).expected(spec["shared"], hidden_size))
         return out
@@ -267,7 +294,13 @@ class RoutedExperts:
             self.correction = tensors[n["correction"]].to(torch.float32).contiguous()
         if self.has_bias:
             self.router_bias = tensors[n["router_bias"]].to(torch.float32).contiguous()
-        if self.E:
+        if self.eight_bit:
+            held = held_tensors({n[k].format(e) + s: tensors[n[k].format(e) + s] for e in range(self.E) for k in ("gate", "up", "down")
+                                 for s in ("", "_scale_inv")})
+            self.w_gate_up = kernels_fp8.stack_matrices([kernels_fp8.gate_up_matrix(held[n["gate"].format(e)], held[n["up"].format(e)])
+                                                         for e in range(self.E)])
+            self.w_down = kernels_fp8.stack_matrices([held[n["down"].format(e)] for e in range(self.E)])
+        elif self.E:
             mats = [tensors[n[k].format(e)] for e in range(self.E) for k in ("gate", "up", "down")]
             common = torch.float32 if any(m.dtype == torch.float32 for m in mats) else mats[0].dtype
             # per expert: eight gate rows and the eight up rows of the same outputs in turn (the layout
@@ -284,12 +317,11 @@ class RoutedExperts:
             self.w_down = torch.stack([tensors[n["down"].format(e)].to(common) for e in range(self.E)]).contiguous()
 
     def weights(self):
-        own = tuple(t for t in (self.w_router, self.correction, self.router_bias, self.w_gate_up, self.w_down)
-                    if t is not None)
+        own = tuple(flat_weights(self.w_router, self.correction, self.router_bias, self.w_gate_up, self.w_down))
         return own + (tuple(self.shared.weights()) if self.shared is not None else ())
 
     def notices(self) -> list:
-        if self.w_gate_up is not None and self.dtype == torch.bfloat16 and \
+        if self.w_gate_up is not None and self.dtype == torch.bfloat16 and not self.eight_bit and \
                 (self.w_gate_up.dtype != torch.bfloat16 or self.hidden % 8 or self.inter % 8):
             return ["routed experts: matrices kept in 32-bit, or sizes that are no multiple of 8: their "
                     "products run on the CUDA cores, not on the tensor cores"]
@@ -297,10 +329,13 @@ class RoutedExperts:
 
     def forward(self, h: torch.Tensor, ctx, residual32: torch.Tensor, x_self32: torch.Tensor = None) -> None:
         rows32, pair_row, weight = self._experts(h, ctx)
-        if x_self32 is None and self.I:
-            x_self32 = h if h.dtype == torch.float32 else h.float()
-        kernels.moe_combine(rows32, pair_row, weight, x_self32 if self.I else rows32, self.top, residual32,
-                            accumulate=True)
+        if self.eight_bit and self.hidden % 4 == 0:
+            kernels.moe_back(rows32, pair_row, weight, h if x_self32 is None else x_self32, residual32, accumulate=True)
+        else:
+            if x_self32 is None and self.I:
+                x_self32 = h if h.dtype == torch.float32 else h.float()
+            kernels.moe_combine(rows32, pair_row, weight, x_self32 if self.I else rows32, self.top, residual32,
+                                accumulate=True)
         if self.shared is not None:
             self.shared.forward(h, ctx, residual32)
 
@@ -308,9 +343,12 @@ class RoutedExperts:
         """Stores the result.  ``x_self32``: the input in 32-bit, for the experts whose output is their
         input (default: ``h`` widened)."""
         rows32, pair_row, weight = self._experts(h, ctx)
-        if x_self32 is None and self.I:
-            x_self32 = h if h.dtype == torch.float32 else h.float()
-        kernels.moe_combine(rows32, pair_row, weight, x_self32 if self.I else rows32, self.top, out32)
+        if self.eight_bit and self.hidden % 4 == 0:
+            kernels.moe_back(rows32, pair_row, weight, h if x_self32 is None else x_self32, out32)
+        else:
+            if x_self32 is None and self.I:
+                x_self32 = h if h.dtype == torch.float32 else h.float()
+            kernels.moe_combine(rows32, pair_row, weight, x_self32 if self.I else rows32, self.top, out32)
         if self.shared is not None:
             self.shared.forward(h, ctx, out32)
 
@@ -348,6 +386,13 @@ class RoutedExperts:
         idx = ws.buffer("moe.idx", (T, top), torch.int32)
         weight = ws.buffer("moe.weight", (T, top), torch.float32)
         n_pairs = T * top
+        if self.eight_bit:
+            kernels.moe_route(z, self.correction, top, self.renormalise, idx, weight, self.scale, self.score, self.groups, self.groups_kept,
+                              self.router_bias)
+            rows32 = ws.buffer("moe.rows", (n_pairs, self.hidden), torch.float32)
+            pair_row = ws.buffer("moe.pair_row", (n_pairs,), torch.int32)
+            kernels.moe_experts_fp8(h, idx, self.w_gate_up, self.w_down, rows32, pair_row, self.form, ws)
+            return rows32, pair_row, weight
         tile = kernels.moe_tile_rows()
         max_tiles = -(-n_pairs // tile) + E               # every expert's last tile may be part full
         plan = ws.buffer("moe.plan", (E + 2 + 3 * max_tiles,), torch.int32)

@@ -41,6 +41,8 @@ inside the root, no weight);
 [heads, hidden]);
 ``pad_heads`` (bfloat16): pages hold heads at the next size that the tensor-core attention kernels take, zero-filled
 (scores and sums are what they were);
+``eight_bit``: the matrices are in 8-bit floating point, a scale for each 128 x 128, and the activations in front of them are quantised
+(``kernels.linear``); in bfloat16 and in float32;
 ``one_pass_prologue``: norm, rotation and page writes in the one kernel below even where the narrower
 kernels would do (a rotation of neighbouring pairs then costs one launch instead of four).
 The first, second, third, sixth, the value norm, the unit norm and the gates take the prologue kernel that
@@ -62,10 +64,12 @@ import math
 
 import torch
 
-from .. import kernels
+from .. import kernels, kernels_fp8
 from ..cache.storage import KVNeed, KVView
 from ..config.specs import ConfigError, PartSpec
+from ..weights.eight_bit import expect_eight_bit
 from ..weights.loader import Expected
+from .eight_bit import flat_weights, held_tensors
 from .fused import normed_linear, normed_rows
 from .registry import norm_class, position_class, register_mixer
 
@@ -87,6 +91,7 @@ class GQAAttention:
             raise ConfigError(f"gqa_attention: head_dim {self.hd} outside 1..512")
         self.dtype, self.device = dtype, device
         self.names = dict(spec["names"])
+        self.eight_bit = bool(spec.get("eight_bit") or False)
         qk = spec.get("qk_norm")
         self.qk_eps = 0.0
         self.has_qk_norm = qk is not None
@@ -167,22 +172,29 @@ class GQAAttention:
             out[n["gate"]] = Expected((spec["n_heads"] if spec["out_gate"] == "head_sigmoid" else no, hidden_size))
         if spec.get("sink") == "learned":
             out[n["sink"]] = Expected((spec["n_heads"],))
-        return out
+        return expect_eight_bit(out, [n[k] for k in ("q", "k", "v", "o", "gate") if k in n]) if spec.get("eight_bit") else out
 
     def bind(self, tensors: dict) -> None:
         n = self.names
+        if self.eight_bit:
+            tensors = held_tensors(tensors)
         parts = [tensors[n["q"]]] if self.shared_kv else \
             [tensors[n["q"]], tensors[n["k"]], tensors[n["v"]]]
         if self.out_gate:
             parts.append(tensors[n["gate"]])          # reads the same input: one product
         if self.has_bias:
             self.bias = torch.cat([tensors[n[k]].to(torch.float32) for k in ("q_bias", "k_bias", "v_bias")]).contiguous()
-        common = torch.float32 if any(p.dtype == torch.float32 for p in parts) else parts[0].dtype
         pad = -sum(p.shape[0] for p in parts) % 8 if self.wide else 0
-        if pad:                                       # an output row then starts on 16 bytes in bfloat16
-            parts.append(torch.zeros((pad, self.hidden), dtype=common, device=parts[0].device))
-        self.w_qkv = torch.cat([p.to(common) for p in parts], dim=0).contiguous()
-        self.w_o = tensors[n["o"]].contiguous()
+        if self.eight_bit:
+            if pad:
+                parts.append(kernels_fp8.quantize_matrix(torch.zeros((pad, self.hidden), device=parts[0].q.device)))
+            self.w_qkv, self.w_o = kernels_fp8.side_by_side(parts), tensors[n["o"]]
+        else:
+            common = torch.float32 if any(p.dtype == torch.float32 for p in parts) else parts[0].dtype
+            if pad:                                   # an output row then starts on 16 bytes in bfloat16
+                parts.append(torch.zeros((pad, self.hidden), dtype=common, device=parts[0].device))
+            self.w_qkv = torch.cat([p.to(common) for p in parts], dim=0).contiguous()
+            self.w_o = tensors[n["o"]].contiguous()
         if self.learned_sink:
             self.sink = tensors[n["sink"]].to(torch.float32).contiguous()
         if self.has_qk_norm:
@@ -191,7 +203,7 @@ class GQAAttention:
                 self.k_norm_w = tensors[n["k_norm"]].to(torch.float32).contiguous()
 
     def weights(self):
-        return [t for t in (self.w_qkv, self.w_o, self.q_norm_w, self.k_norm_w, self.bias, self.sink) if t is not None]
+        return flat_weights(self.w_qkv, self.w_o, self.q_norm_w, self.k_norm_w, self.bias, self.sink)
 
     def absorb_norm_weight(self, norm) -> bool:
         """Takes the weight of the norm in front of this mixer into the columns of the q/k/v
@@ -351,8 +363,8 @@ class DiffAttention(GQAAttention):
         self.H, self.G = int(spec["n_heads"]), int(spec["n_kv_heads"])
         params = spec.as_dict()
         params.update(n_heads=2 * self.H, n_kv_heads=2 * self.G, one_pass_prologue=True)
-        if spec.get("shared_kv") or spec.get("out_gate") or spec.get("pool"):
-            raise ConfigError("diff_attention: neither shared_kv nor an output gate nor pooled blocks")
+        if spec.get("shared_kv") or spec.get("out_gate") or spec.get("pool") or spec.get("eight_bit"):
+            raise ConfigError("diff_attention: neither shared_kv nor an output gate nor pooled blocks nor matrices in 8 bits")
         super().__init__(PartSpec.make("gqa_attention", **params), hidden_size, dtype, device)
         self.n_v_heads = self.G
         self.diff = float(spec["diff"])

@@ -30,11 +30,13 @@ class FreeSize(int):
 @dataclass(frozen=True)
 class Expected:
     """A tensor the model needs.  ``init`` tells the random-weights writer how to fill
-    it: "matrix" (N(0, std)), "scale" (1 + N(0, scale_std)) or "mixing" (the identity + N(0, scale_std)).  ``optional`` tensors may
-    be absent (an lm_head matrix beside tied embeddings)."""
+    it: "matrix" (N(0, std)), "scale" (1 + N(0, scale_std)), "mixing" (the identity + N(0, scale_std)) or "block_scales" (of the matrix in front
+    of it, which is in 8 bits).  ``optional`` tensors may be absent (an lm_head matrix beside tied embeddings).  ``eight_bit``: a matrix of F8_E4M3,
+    and only that."""
     shape: tuple
     init: str = "matrix"
     optional: bool = False
+    eight_bit: bool = False
 
 
 def runtime_dtype(stored: torch.dtype, compute: torch.dtype) -> torch.dtype:
@@ -89,13 +91,17 @@ def load_weights(folder, expected: Mapping[str, Expected], compute_dtype: torch.
         if dup:
             raise WeightsError("tensors present in more than one shard: " + ", ".join(sorted(dup)))
         check_names_and_shapes(expected, {n: f.entries[n].shape for n, f in where.items()})
+        odd = [f"    {n}  has unsupported dtype {f.entries[n].dtype}, expected {'F8_E4M3' if expected[n].eight_bit else 'one of more than 8 bits'}"
+               for n, f in where.items() if (f.entries[n].dtype == "F8_E4M3") != expected[n].eight_bit]
+        if odd:
+            raise WeightsError("\n".join([f"weights do not match the model:\n  wrong type ({len(odd)}), by quantization_config of config.json:"] + odd))
         out = {}
         for name in expected:
             if name not in where:
                 continue
             cpu = where[name].tensor(name)
-            out[name] = cpu.to(device=device, dtype=runtime_dtype(cpu.dtype, compute_dtype),
-                               copy=True)
+            kept = cpu.dtype if expected[name].eight_bit else runtime_dtype(cpu.dtype, compute_dtype)
+            out[name] = cpu.to(device=device, dtype=kept, copy=True)
             del cpu
         return out
     finally:

@@ -23,6 +23,7 @@ from typing import Mapping
 import numpy as np
 import torch
 
+from .eight_bit import F8, held, scale_name
 from .loader import Expected, runtime_dtype
 from .safetensors_io import write_safetensors
 
@@ -139,14 +140,17 @@ def random_tensors_on_device(expected: Mapping[str, Expected], seed: int, storag
                              scale_std: float = 0.1) -> dict:
     """name -> tensor on ``device`` for every non-optional expected tensor: generated in the
     storage dtype (what a written folder would hold), kept in the dtype the loader would
-    give it under ``compute``."""
+    give it under ``compute``.  A matrix in 8 bits is the one that would be there otherwise, quantised."""
     tensors = {}
     for i, (name, e) in enumerate(expected.items()):
-        if e.optional:
+        if e.optional or e.init == "block_scales":       # (made with their matrix)
             continue
         t = torch.empty(tuple(e.shape), dtype=storage, device=device)
         fill_random_on_device(t, e, seed, i, std, scale_std)
-        tensors[name] = t.to(runtime_dtype(storage, compute))
+        if e.eight_bit:
+            tensors[name], tensors[scale_name(name)] = held(t)
+        else:
+            tensors[name] = t.to(runtime_dtype(storage, compute))
     return tensors
 
 
@@ -180,9 +184,23 @@ def write_random_model(folder, config: Mapping, seed: int, dtype: str = "bfloat1
         fill_random_on_device(t, e, seed, i, std, scale_std)
         return t.cpu()
 
+    made: dict = {}              # a matrix in 8 bits' scales, between its turn and theirs
+
+    def make_eight_bit(name, e, i):
+        t = make(e, i)
+        q, made[scale_name(name)] = held(t.cuda() if on_device else t)
+        made[scale_name(name)] = made[scale_name(name)].cpu()
+        return q.cpu()
+
     items = []
     for i, (name, e) in enumerate(expected.items()):
         if e.optional:
+            continue
+        if e.eight_bit:
+            items.append((name, tuple(e.shape), F8, (lambda name=name, e=e, i=i: make_eight_bit(name, e, i))))
+            continue
+        if e.init == "block_scales":
+            items.append((name, tuple(e.shape), torch.float32, (lambda name=name: made.pop(name))))
             continue
         items.append((name, tuple(e.shape), tdtype, (lambda e=e, i=i: make(e, i))))
     write_safetensors(folder / "model.safetensors", items)

@@ -25,7 +25,7 @@ class WeightsError(RuntimeError):
 _TORCH_DTYPE = {
     "F32": torch.float32, "F16": torch.float16, "BF16": torch.bfloat16, "F64": torch.float64,
     "I64": torch.int64, "I32": torch.int32, "I16": torch.int16, "I8": torch.int8,
-    "U8": torch.uint8, "BOOL": torch.bool,
+    "U8": torch.uint8, "BOOL": torch.bool, "F8_E4M3": torch.float8_e4m3fn,
 }
 _ST_NAME = {v: k for k, v in _TORCH_DTYPE.items()}
 
@@ -90,8 +90,9 @@ class SafetensorsFile:
             n *= s
         if n == 0:
             return torch.empty(e.shape, dtype=_TORCH_DTYPE[e.dtype])
-        t = torch.frombuffer(self._map, dtype=_TORCH_DTYPE[e.dtype], count=n, offset=e.begin)
-        return t.reshape(e.shape)
+        dtype = _TORCH_DTYPE[e.dtype]
+        t = torch.frombuffer(self._map, dtype=torch.uint8 if dtype.itemsize == 1 else dtype, count=n, offset=e.begin)
+        return (t.view(dtype) if dtype.itemsize == 1 else t).reshape(e.shape)
 
     def close(self) -> None:
         # views handed out keep the map alive through the buffer protocol; closing
