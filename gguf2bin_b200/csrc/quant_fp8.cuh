@@ -167,7 +167,7 @@ static int run_quantize_matrix(const void *w, int dtype, int count, int N, int K
 constexpr int SORT_WARPS = 32, SORT_MOST_EXPERTS = 1024, SORT_AHEAD = 8;
 
 // One block.  A warp takes a stretch of the pairs, 32 at a time: lanes with one expert find each other (a ballot a bit of its number: match.any
-// takes 48 cycles of the multiprocessor, 27 us for 16,384 pairs; this 9), the first of them counts for all.  No two warps share a counter, so
+// takes 48 cycles of the multiprocessor: 27 us for 16,384 pairs, where this takes 12), the first of them counts for all.  No two warps share a counter, so
 // nothing depends on who comes first.  A pair's place among its warp's waits in pair_row for the rows in front of it.
 __global__ void __launch_bounds__(SORT_WARPS * 32)
 moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int bits, int *__restrict__ starts, int *pair_row, int *__restrict__ row_pair) {
