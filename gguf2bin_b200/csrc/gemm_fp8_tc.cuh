@@ -32,16 +32,16 @@ constexpr int ADDER_REGS = 232, OTHER_REGS = 40;
 constexpr int COLS = BN / 2, PIECE = 16;
 constexpr int RING_BYTES = STAGES * STAGE_BYTES;
 constexpr int BOX_BYTES = 32 * 128;                      // an adder's outputs on their way to C: 32 rows of 128 bytes, swizzled as the ring is
-constexpr int BAR_BYTES = 256, LIST_BYTES = MOST_EXPERTS * 4;
+constexpr int BAR_BYTES = 256, TILE_BYTES = ADDERS * 16, LIST_BYTES = (2 * MOST_EXPERTS + 4) * 4;
 // Boxes of an adder: two where there is room, so that one is filled while the other is written out.
 template <bool GROUPED> constexpr int BOXES = GROUPED ? 1 : 2;
 template <bool GROUPED>
-constexpr int SMEM = RING_BYTES + ADDERS * BOXES<GROUPED> * BOX_BYTES + BAR_BYTES + (GROUPED ? LIST_BYTES : 0) + 1024;      // + the swizzle's alignment
+constexpr int SMEM = RING_BYTES + ADDERS * BOXES<GROUPED> * BOX_BYTES + BAR_BYTES + TILE_BYTES + (GROUPED ? LIST_BYTES : 0) + 1024;      // + the swizzle's alignment
 static_assert(SMEM<false> <= 227 * 1024 && SMEM<true> <= 227 * 1024, "one CTA a multiprocessor");
 constexpr int BAND = 8;                                  // tiles along M that are walked side by side
 
 struct Tc : Product {
-  int nb, boxes;                                         // nb: blocks of W's rows that have a scale; boxes: map_out may be used
+  int nb, boxes, silu;                                   // nb: blocks of W's rows that have a scale; boxes: map_out may be used; silu: form is the plain one
 };
 
 template <bool ACC>
@@ -69,7 +69,7 @@ constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)
 
 struct Tile { int e, m0, end, n0; };
 
-// Tile t of the walk.  `list`: with experts, list[e] = tiles of the experts up to e along M (in shared memory).
+// Tile t of the walk.  `list` (in shared memory): with experts, list[e] = tiles of the experts up to e along M, and behind them p.starts.
 template <bool GROUPED>
 __device__ __forceinline__ Tile find_tile(const Tc &p, const int *list, int t, int tiles_n) {
   Tile r;
@@ -81,7 +81,7 @@ __device__ __forceinline__ Tile find_tile(const Tc &p, const int *list, int t, i
       else lo = mid + 1;
     }
     const int before = lo ? list[lo - 1] : 0, high = list[lo] - before, at = t - before * tiles_n;
-    r.e = lo, r.n0 = at / high * BN, r.m0 = p.starts[lo] + at % high * 2 * BM, r.end = p.starts[lo + 1];
+    r.e = lo, r.n0 = at / high * BN, r.m0 = list[MOST_EXPERTS + lo] + at % high * 2 * BM, r.end = list[MOST_EXPERTS + lo + 1];
   } else {
     const int tiles_m = (p.M + 2 * BM - 1) / (2 * BM), band = t / (BAND * tiles_n), high = min(BAND, tiles_m - band * BAND), at = t - band * BAND * tiles_n;
     r.e = 0, r.n0 = at / high * BN, r.m0 = (band * BAND + at % high) * 2 * BM, r.end = p.M;
@@ -103,7 +103,8 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
   // adder has seen it before the stage's next products are issued).  A commit costs the tensor cores about 200 cycles: one a block, not two.
   const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * STAGES, sum_empty0 = done0 + 8 * STAGES;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2);
-  int *list = reinterpret_cast<int *>(smem + RING_BYTES + OUT_BYTES + BAR_BYTES);
+  int4 *tiles = reinterpret_cast<int4 *>(smem + RING_BYTES + OUT_BYTES + BAR_BYTES);      // an adding warp's tile: its first row, end, first column
+  int *list = reinterpret_cast<int *>(tiles + ADDERS);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t half = cluster_ctarank();               // the pair's first CTA issues its products
   if (threadIdx.x == 0) {
@@ -122,8 +123,10 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     if (warp == 0) {                                     // tiles of the experts, summed up 32 at a time
       int sum = 0;
       for (int e0 = 0; e0 < p.n_experts; e0 += 32) {
-        const int e = e0 + lane;
-        int v = e < p.n_experts ? (p.starts[e + 1] - p.starts[e] + 2 * BM - 1) / (2 * BM) : 0;
+        const int e = e0 + lane, first = p.starts[min(e, p.n_experts)], behind = p.starts[min(e + 1, p.n_experts)];
+        int v = (behind - first + 2 * BM - 1) / (2 * BM);
+        if (e <= p.n_experts) list[MOST_EXPERTS + e] = first;
+        if (e + 1 == p.n_experts) list[MOST_EXPERTS + e + 1] = behind;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int u = __shfl_up_sync(0xffffffffu, v, o);
@@ -204,21 +207,27 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     int box = 0;
     bool ok = true;                                      // once a wait gave up nothing is waited for any more, and (but with EPI_GATED_ROWS, whose warps
     int it = 0;                                          // meet in pairs at every tile) nothing is written
+    // Inside the loop over K the sums and the pieces of an accumulator take 160 of the 232 registers and addresses most of the rest: the tile waits in
+    // shared memory, and the scales' places are 32-bit offsets.  A tile's first scales are asked for in front of the last one's outputs.
+    int at_a = 0, at_w = 0;
+    float next_a = 0.f, next_w = 0.f, next_up = 0.f;
+    auto begin = [&](int t) {
+      const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
+      const int m0 = tile.m0 + (int)half * BM + row0;
+      at_a = min(m0 + lane, p.M - 1);
+      // the thread's columns are one block of W's rows; gated, one of the gate's and one of the up's
+      const int n_block = GATED ? tile.n0 / 2 / F8_BLOCK : min((tile.n0 + col0) / F8_BLOCK, p.nb - 1);
+      at_w = (tile.e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks;
+      next_a = p.sa[at_a], next_w = p.sw[at_w], next_up = GATED ? p.sw[at_w + p.nb * p.blocks] : 0.f;
+      __syncwarp();
+      if (lane == 0) tiles[warp] = make_int4(m0, tile.end, tile.n0, 0);
+      __syncwarp();
+    };
+    if (pair < n_tiles) begin(pair);
     for (int t = pair; t < n_tiles; t += pairs) {
-      // Inside the loop over K the sums and the pieces of an accumulator take 160 of the 232 registers and addresses most of
-      // the rest: the tile is found again behind it, and the scales' places are 32-bit offsets.
-      int at_a, at_w;
-      {
-        const Tile tile = find_tile<GROUPED>(p, list, t, tiles_n);
-        at_a = min(tile.m0 + (int)half * BM + row0 + lane, p.M - 1);
-        // the thread's columns are one block of W's rows; gated, one of the gate's and one of the up's
-        const int n_block = GATED ? tile.n0 / 2 / F8_BLOCK : min((tile.n0 + col0) / F8_BLOCK, p.nb - 1);
-        at_w = (tile.e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks;
-      }
       float sum[COLS];
 #pragma unroll
       for (int j = 0; j < COLS; ++j) sum[j] = 0.f;
-      float next_a = p.sa[at_a], next_w = p.sw[at_w], next_up = GATED ? p.sw[at_w + p.nb * p.blocks] : 0.f;
       for (int b = 0; b < p.blocks; ++b, ++it) {
         const int h = it & 1;
         const float f = next_a * next_w, f_up = next_a * next_up;
@@ -263,38 +272,53 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
       }
       if (!ok && EPI != EPI_GATED_ROWS) break;
-      int again = t;
-      asm volatile("" : "+r"(again));
-      const Tile tile = find_tile<GROUPED>(p, list, again, tiles_n);
-      const int m0 = tile.m0 + (int)half * BM + row0;
-      const int rows = min(32, tile.end - m0);           // of this warp's that exist (may be none)
+      const int4 tile = tiles[warp];
+      const int m0 = tile.x, n0 = tile.z;
+      if (t + pairs < n_tiles) begin(t + pairs);
+      const int rows = min(32, tile.y - m0);           // of this warp's that exist (may be none)
       if (GATED) {
-        const int n_out = p.N / 2, out0 = (tile.n0 + col0) / 2;                        // 64 outputs a thread
-        float most = 0.f;
+        const int n_out = p.N / 2, out0 = (n0 + col0) / 2;                        // 64 outputs a thread
+        [[maybe_unused]] float most = 0.f;
+        if (p.silu) {
 #pragma unroll
-        for (int j = 0; j < COLS / 2; ++j) {
-          const int c = (j >> 3) * 16 + (j & 7);
-          float v = glu_value_fast(sum[c], sum[c + 8], p.form);
-          if (out0 + j >= n_out) v = 0.f;
-          sum[j] = v;
-          most = max_nan(most, fabsf(v));
+          for (int j = 0; j < COLS / 2; ++j) sum[j] = silu_value_fast(sum[(j >> 3) * 16 + (j & 7)], sum[(j >> 3) * 16 + (j & 7) + 8]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < COLS / 2; ++j) sum[j] = glu_value_fast(sum[(j >> 3) * 16 + (j & 7)], sum[(j >> 3) * 16 + (j & 7) + 8], p.form);
         }
+        if (out0 + COLS / 2 > n_out)                     // the last outputs' tile: zeros behind them
+#pragma unroll
+          for (int j = 0; j < COLS / 2; ++j)
+            if (out0 + j >= n_out) sum[j] = 0.f;
         if (EPI == EPI_GATED_ROWS) {
-          float *const given = reinterpret_cast<float *>(boxes);       // the largest of a row: of the two warps that share it
+          float *const given = reinterpret_cast<float *>(boxes + BOX_BYTES / 2);       // the largest of a row: of the two warps that share it
+#pragma unroll
+          for (int j = 0; j < COLS / 2; ++j) most = max_nan(most, fabsf(sum[j]));
           given[lane] = most;
           asm volatile("bar.sync %0, 64;\n" ::"r"(1 + warp % 4) : "memory");
           most = max_nan(most, (given + (warp < 4 ? 4 : -4) * BOXES<GROUPED> * BOX_BYTES / 4)[lane]);
           const BlockScale s = block_scale(most);
-          if (lane < rows) {
-            if (warp < 4) p.out_scale[tile.n0 / 2 / F8_BLOCK * p.ldos + m0 + lane] = s.scale;
-            uint8_t *to = static_cast<uint8_t *>(p.out) + (long long)(m0 + lane) * p.ldo + out0;
+          if (lane < rows && warp < 4) p.out_scale[n0 / 2 / F8_BLOCK * p.ldos + m0 + lane] = s.scale;
+          // 64 bytes a row, in rows through a box (the copy unit does not know an expert's last row, so there lanes write their own)
+          const bool copied = p.boxes && (!GROUPED || rows == 32);
+          if (copied && lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+          uint8_t *const to = static_cast<uint8_t *>(p.out) + (long long)(m0 + lane) * p.ldo + out0;
 #pragma unroll
-            for (int j = 0; j < COLS / 2; j += 16) {
-              uint32_t w[4];
+          for (int j = 0; j < COLS / 2; j += 16) {
+            uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                w[i] = pack_e4m3(sum[j + 4 * i] * s.inverse, sum[j + 4 * i + 1] * s.inverse, sum[j + 4 * i + 2] * s.inverse, sum[j + 4 * i + 3] * s.inverse);
-              *reinterpret_cast<uint4 *>(to + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i)
+              w[i] = pack_e4m3(sum[j + 4 * i] * s.inverse, sum[j + 4 * i + 1] * s.inverse, sum[j + 4 * i + 2] * s.inverse, sum[j + 4 * i + 3] * s.inverse);
+            if (copied) *reinterpret_cast<uint4 *>(boxes + lane * 64 + ((j / 16 ^ (lane >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            else if (lane < rows) *reinterpret_cast<uint4 *>(to + j) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (copied) {
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && rows > 0) {
+              tma_store_2d(&map_out, smem_addr(boxes), out0, m0);
+              bulk_commit();
             }
           }
           asm volatile("bar.sync %0, 64;\n" ::"r"(1 + warp % 4) : "memory");     // the next tile's largest go where this one's were
@@ -305,12 +329,12 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       // 32 rows of 128 bytes at a time through a box: written out (or added to what is there: every output gets one addition) by the copy unit,
       // or, where C's rows do not start on 16 bytes or some of the rows are another expert's, read back by the warp, eight lanes a row.
       constexpr int OUTS = GATED ? COLS / 2 : COLS, WIDE = EPI == EPI_BF16 ? 64 : 32;
-      const int n_out = GATED ? p.N / 2 : p.N, first = GATED ? (tile.n0 + col0) / 2 : tile.n0 + col0;
+      const int n_out = GATED ? p.N / 2 : p.N, first = GATED ? (n0 + col0) / 2 : n0 + col0;
       const bool copied = p.boxes && (!GROUPED || rows == 32);
 #pragma unroll
       for (int q = 0; q < OUTS / WIDE; ++q) {
-        const int n0 = first + WIDE * q;
-        if (n0 >= n_out) break;
+        const int n1 = first + WIDE * q;
+        if (n1 >= n_out) break;
         int l = lane;
         asm volatile("" : "+r"(l));                      // or the boxes' addresses are kept over the loop above
         unsigned char *const at = boxes + box * BOX_BYTES;
@@ -338,15 +362,15 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
           fence_async_shared();
           __syncwarp();
           if (lane == 0) {
-            if (EPI == EPI_ADD_F32) tma_reduce_add_2d(&map_out, smem_addr(at), n0, m0);
-            else tma_store_2d(&map_out, smem_addr(at), n0, m0);
+            if (EPI == EPI_ADD_F32) tma_reduce_add_2d(&map_out, smem_addr(at), n1, m0);
+            else tma_store_2d(&map_out, smem_addr(at), n1, m0);
             bulk_commit();
           }
         } else {
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + lane / 8, j = lane % 8, n = n0 + WIDE / 8 * j;
+            const int r = 4 * i + lane / 8, j = lane % 8, n = n1 + WIDE / 8 * j;
             if (r >= rows) break;
             const uint4 w = *reinterpret_cast<const uint4 *>(at + r * 128 + ((j ^ (r & 7)) << 4));
             const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -410,10 +434,13 @@ static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, Tc p, cuda
   if (((long long)p.M / (2 * BM) + 1 + (GROUPED ? p.n_experts : 0)) * tiles_n > INT32_MAX) G2B_REFUSE("gemm_fp8_tc: %d x %d is too large for one launch", p.M, p.N);
   const int pairs = (int)(tiles < most ? tiles : most);
   CUtensorMap map_out = map_a;
-  constexpr int SIZE = EPI == EPI_BF16 ? 2 : 4;
-  p.boxes = EPI != EPI_GATED_ROWS && p.ldo * SIZE % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldo <= INT32_MAX;
-  if (p.boxes) {
-    const int rc = get_map(&map_out, p.out, p.M, EPI == EPI_GATED_F32 ? p.N / 2 : p.N, (int)p.ldo, 32, SIZE);
+  constexpr bool ROWS = EPI == EPI_GATED_ROWS;
+  constexpr int SIZE = ROWS ? 1 : EPI == EPI_BF16 ? 2 : 4;
+  p.boxes = p.ldo * SIZE % 16 == 0 && ((uintptr_t)p.out & 15) == 0 && p.ldo <= INT32_MAX;
+  p.silu = p.form.limit == INFINITY && p.form.offset == 0.f && p.form.c1 == 1.f && p.form.c3 == 0.f;
+  if (p.boxes) {                                         // (quantised rows go to their blocks' ends, zeros included)
+    const int columns = ROWS ? (p.N / 2 + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK : EPI == EPI_GATED_F32 ? p.N / 2 : p.N;
+    const int rc = get_map(&map_out, p.out, p.M, columns, (int)p.ldo, 32, SIZE, ROWS ? 64 : 128);
     if (rc) G2B_REFUSE("gemm_fp8_tc: cuTensorMapEncodeTiled failed (%d)", rc);
   }
   g2b_launch_cluster(gemm_fp8_tc_kernel<EPI, GROUPED>, dim3(2 * pairs), dim3(THREADS), (size_t)SMEM<GROUPED>, stream, 2u, map_a, map_w, map_out, p);

@@ -22,6 +22,9 @@ __device__ __forceinline__ float glu_value_fast(float gate, float up, const GluF
   return __fdividef(g, 1.f + __expf(-(g * fmaf(f.c3 * g, g, f.c1)))) * u;
 }
 
+// The plain form by itself: SiLU(gate) * up, a third of the operations.
+__device__ __forceinline__ float silu_value_fast(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
+
 // The activation alone: z * sigmoid(z (c1 + c3 z^2)).
 __device__ __forceinline__ float act_value(float z, const GluForm &f) { return z / (1.f + expf(-(z * fmaf(f.c3 * z, z, f.c1)))); }
 __device__ __forceinline__ float act_value_fast(float z, const GluForm &f) {

@@ -370,31 +370,31 @@ static inline EncodeTiledFn encode_fn() {
 }
 
 struct MapKey {
-  const void *base; long long rows; int cols, ld, box_rows, elem_bytes;
+  const void *base; long long rows; int cols, ld, box_rows, elem_bytes, box_bytes;
   bool operator==(const MapKey &o) const {
     return base == o.base && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows &&
-           elem_bytes == o.elem_bytes;
+           elem_bytes == o.elem_bytes && box_bytes == o.box_bytes;
   }
 };
 struct MapKeyHash {
   size_t operator()(const MapKey &k) const {
     size_t h = std::hash<const void *>()(k.base);
     h = h * 1000003u ^ (size_t)k.rows; h = h * 1000003u ^ (size_t)k.cols;
-    h = h * 1000003u ^ (size_t)k.ld;   h = h * 1000003u ^ (size_t)(k.box_rows * 8 + k.elem_bytes);
+    h = h * 1000003u ^ (size_t)k.ld;   h = h * 1000003u ^ (size_t)(k.box_rows * 8 + k.elem_bytes + (k.box_bytes << 16));
     return h;
   }
 };
 
 // A tiled map of a row-major [rows, cols] matrix of bytes (elem_bytes 1), bfloat16 (2) or float (4), row
-// stride ld elements, with boxes of box_rows rows x 128 bytes and 128-byte swizzle; parts of a
+// stride ld elements, with boxes of box_rows rows x 128 bytes and 128-byte swizzle (or x 64 and 64-byte); parts of a
 // box outside the matrix read as zero and are not written.  Encoded maps are kept by (address,
 // sizes): weights, cache layers and scratch buffers come back with the same values every step.
 // Returns 0, or a CUresult / -1 on failure.
 static inline int get_map(CUtensorMap *map, const void *base, long long rows, int cols, int ld,
-                          int box_rows, int elem_bytes = 2) {
+                          int box_rows, int elem_bytes = 2, int box_bytes = 128) {
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> maps;
   static std::mutex mutex;
-  const MapKey key{base, rows, cols, ld, box_rows, elem_bytes};
+  const MapKey key{base, rows, cols, ld, box_rows, elem_bytes, box_bytes};
   std::lock_guard<std::mutex> lock(mutex);
   auto it = maps.find(key);
   if (it != maps.end()) {
@@ -405,13 +405,13 @@ static inline int get_map(CUtensorMap *map, const void *base, long long rows, in
   if (!fn) return -1;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * (cuuint64_t)elem_bytes};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / elem_bytes), (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)(box_bytes / elem_bytes), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, elem_bytes == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                        : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                          : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2,
                   const_cast<void *>(base), dims, strides,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return (int)r;
   if (maps.size() > 65536) maps.clear();               // a bound, not a policy: maps are cheap to rebuild

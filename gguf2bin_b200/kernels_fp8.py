@@ -64,11 +64,8 @@ def _plan(key, call: _Call, device, prepare: str, name: str, argtypes, x_aligned
     return plan
 
 
-def _launched(plan: _Plan, n: int) -> None:
-    """What a function of several launches returned: how many, or less than zero for an error."""
-    if n < 0:
-        raise KernelError(plan.f._lib.g2b_last_error().decode("utf-8", "replace"))
-    kernels.count_launches(n)
+def _failed(f) -> None:
+    raise KernelError(f._lib.g2b_last_error().decode("utf-8", "replace"))
 
 
 def _scratch(plan: _Plan, workspace, name: str, device):
@@ -140,7 +137,7 @@ def quantize_rows(x: torch.Tensor, rows: Fp8Rows, pair_row: Optional[torch.Tenso
     rc = f(x.data_ptr(), *given[0], q.data_ptr(), given[1], scale.data_ptr(), given[2], None if pair_row is None else pair_row.data_ptr(), given[3], given[4],
            _stream())
     if rc:
-        raise KernelError(f._lib.g2b_last_error().decode("utf-8", "replace"))
+        _failed(f)
     kernels.count_launches(1)
 
 
@@ -263,18 +260,34 @@ def _plan_product(key, what: str, a, w: Fp8Matrix, out, epi: int, form, columns:
 def _product(what: str, a, w: Fp8Matrix, out, epi: int, form=SILU, workspace=None, columns: int = BY_THE_RULE, split: int = 1, defines=()) -> None:
     """``columns`` and ``split``: the tiles of ``gemm_fp8_few.cuh`` and the parts of K (``BY_THE_RULE``: what ``choose`` in products_fp8.cu says)."""
     q, s, k = w
-    given, as_rows = isinstance(a, Fp8Rows), isinstance(out, Fp8Rows)
-    key = (_seen(a.q) + _seen(a.scale) if given else _seen(a), _seen(q), _seen(s), k, _seen(out.q) + _seen(out.scale) if as_rows else _seen(out), epi, form,
-           _here(), columns, split, defines)
-    plan = _plans.get(key) or _plan_product(key, what, a, w, out, epi, form, columns, split, defines)
-    scratch, held = _scratch(plan, workspace, "fp8.product", q.device)
-    n = plan.f(plan.at, a.q.data_ptr() if given else a.data_ptr(), a.scale.data_ptr() if given else None, scratch, q.data_ptr(), s.data_ptr(),
-               out.q.data_ptr() if as_rows else out.data_ptr(), out.scale.data_ptr() if as_rows else None, plan.status, _stream())
-    _launched(plan, n)
+    if a.__class__ is Fp8Rows:
+        x, x_scale = a
+        seen = _seen(x_scale)
+    else:
+        x, x_scale, seen = a, None, None
+    if out.__class__ is Fp8Rows:
+        to, to_scale = out
+        seen = (seen, _seen(to_scale))
+    else:
+        to, to_scale = out, None
+    at_x, at_q, at_to = x.data_ptr(), q.data_ptr(), to.data_ptr()
+    key = (x.shape, x.stride(), x.dtype, x.get_device(), at_x & 15, q.shape, q.stride(), q.dtype, q.get_device(), at_q & 15, s.shape, s.stride(), s.dtype,
+           s.get_device(), to.shape, to.stride(), to.dtype, to.get_device(), at_to & 15, k, seen, epi, form, _here(), columns, split, defines)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _plan_product(key, what, a, w, out, epi, form, columns, split, defines)
+    scratch = held = None
+    if plan.scratch or workspace is not None:
+        scratch, held = _scratch(plan, workspace, "fp8.product", q.device)
+    n = plan.f(plan.at, at_x, None if x_scale is None else x_scale.data_ptr(), scratch, at_q, s.data_ptr(), at_to,
+               None if to_scale is None else to_scale.data_ptr(), plan.status, _stream())
+    if n < 0:
+        _failed(plan.f)
+    kernels.count_launches(n)
 
 
 def linear(a, w, out: torch.Tensor, accumulate: bool, workspace) -> None:
-    if isinstance(w, Fp8Matrices):
+    if w.__class__ is Fp8Matrices:
         rows, at = a, 0
         _check_out("linear", out, (a.q if isinstance(a, Fp8Rows) else a).shape[0], w.shape[0])
         if not isinstance(a, Fp8Rows):                   # quantised once for all of them
@@ -351,8 +364,11 @@ def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down
     key = (_seen(h), _seen(idx), _seen(gq), _seen(gs), gk, _seen(dq), _seen(ds), dk, _seen(rows32), _seen(pair_row), form, _here())
     plan = _plans.get(key) or _plan_experts(key, h, idx, w_gate_up, w_down, rows32, pair_row, form)
     scratch, held = _scratch(plan, workspace, "fp8.experts", gq.device)
-    _launched(plan, plan.f(plan.at, h.data_ptr(), idx.data_ptr(), scratch, gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(), rows32.data_ptr(),
-                           pair_row.data_ptr(), plan.status, _stream()))
+    n = plan.f(plan.at, h.data_ptr(), idx.data_ptr(), scratch, gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(), rows32.data_ptr(),
+               pair_row.data_ptr(), plan.status, _stream())
+    if n < 0:
+        _failed(plan.f)
+    kernels.count_launches(n)
 
 
 def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool) -> None:
@@ -360,7 +376,7 @@ def moe_back(rows32, pair_row, weight, x_self, out, accumulate: bool) -> None:
     f, given = _plans.get(key) or _plan_back(key, rows32, pair_row, weight, x_self, out, accumulate)
     rc = f(rows32.data_ptr(), pair_row.data_ptr(), weight.data_ptr(), x_self.data_ptr(), *given[0], out.data_ptr(), *given[1], _stream())
     if rc:
-        raise KernelError(f._lib.g2b_last_error().decode("utf-8", "replace"))
+        _failed(f)
     kernels.count_launches(1)
 
 
