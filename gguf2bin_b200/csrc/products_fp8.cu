@@ -29,13 +29,14 @@ struct Choice { int columns, split, with_x; };
 // Microseconds that a product is estimated to take.  With `c` CTAs of `n` blocks of K each, as many as `most` at a time:
 //   start + (parts + part * split, where K is in parts) + the 4-norm of (the rounds of CTAs: n blocks each, and `wave` for every round but one) and
 //   (W's bytes at `rate` TB/s);  a block takes `alone` where no two CTAs share a multiprocessor, else `block`.
-// Fitted to 2,200 times of 150 products (1 to 1,500 rows, 256 to 30,000 outputs, K = 512 to 17,408; graphs of products behind one another): within
-// 6 to 9 % (root mean square of the logarithm); what the estimates choose is 1 % slower than the best choice in the mean, 16 at worst.  With the tiles the
+// Fitted to 7,000 times of 430 products (1 to 1,500 rows, 256 to 30,000 outputs, K = 512 to 17,408; graphs of products behind one another): within
+// 7 to 10 % (root mean square of the logarithm); what the estimates choose is 2 % slower than the best choice in the mean, 26 at worst.  With the tiles the
 // largest that fit instead, 64 rows by 5,120 x 17,408 took 34 us (21), and 128 rows by 6,144 x 4,096 13.9 (11.1).
 struct Cost { double start, parts, part, alone, block, wave, rate; };
-constexpr Cost COST_X = {2.11, 0.62, 0.09, 0.347, 0.345, 2.2, 5.8}, COST_16 = {2.02, 0.57, 0.08, 0.237, 0.320, 1.9, 6.5},
-               COST_32 = {2.50, 0.47, 0.10, 0.272, 0.421, 2.3, 6.8}, COST_64 = {2.60, 0.64, 0.19, 0.361, 0.558, 2.6, 5.2},
-               COST_LANES = {2.69, 0.28, 0.32, 0.276, 0.420, 2.8, 9.4};
+constexpr Cost COST_X = {2.11, 0.60, 0.08, 0.348, 0.408, 1.82, 5.75}, COST_16 = {2.02, 0.59, 0.07, 0.238, 0.349, 1.77, 6.42},
+               COST_32 = {2.57, 0.58, 0.08, 0.280, 0.411, 2.17, 6.46}, COST_64 = {2.81, 0.55, 0.18, 0.357, 0.550, 2.61, 5.27},
+               COST_LANES = {2.89, 0.48, 0.26, 0.271, 0.412, 2.69, 5.67};
+constexpr double MANY_START = 2.41, MANY_BLOCK = 0.430, MANY_TILE = 1.88;   // of gemm_fp8_tc.cuh: a round is its blocks and a tile's outputs
 constexpr double QUANTISED_FIRST = 2.0;                  // a kernel of its own in front
 
 static double estimate(const Cost &k, long long tiles, int blocks, int split, int most, double w_bytes) {
@@ -56,7 +57,7 @@ static Choice choose(int M, int N, int blocks, int experts, bool rows_needed) {
   const long long pairs_tiles = (long long)used * ((each + 255) / 256) * ((N + 255) / 256);
   const int pairs = many::resident();
   Choice best = {0, 1, 0};
-  double least = QUANTISED_FIRST + 2.4 + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * 0.418 + 1.9);
+  double least = QUANTISED_FIRST + MANY_START + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * MANY_BLOCK + MANY_TILE);
   auto look = [&](int columns, bool x, const Cost &k, int (*resident)(int)) {
     const int rows_a = columns > 0 ? columns : 128, rows_w = columns > 0 ? 128 : 64;
     const long long tiles = (long long)used * ((each + rows_a - 1) / rows_a) * ((N + rows_w - 1) / rows_w);
