@@ -26,13 +26,3 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;\n" : "=h"(hi) : "f"(c), "f"(d));
   return (uint32_t)hi << 16 | lo;
 }
-
-// D (16x8, f32) += A (16x32, e4m3, row) * B (32x8, e4m3, col); with g = lane / 4, c = lane % 4 and four values a register
-//   a0 = A[g][4c..]  a1 = A[g+8][4c..]  a2 = A[g][4c+16..]  a3 = A[g+8][4c+16..]   b0 = B[4c..][g]  b1 = B[4c+16..][g]
-//   d0,d1 = D[g][2c,2c+1]  d2,d3 = D[g+8][2c,2c+1]
-__device__ __forceinline__ void mma_e4m3_16832(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}

@@ -124,10 +124,46 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       for (int b = 0; b < CHUNK; ++b) mbar_init(scaled0 + 8 * b, 4);
     mbar_init_fence();
   }
-  int e = 0, m0 = tile_m * S::ROWS_A, end = p.M;
+  int e = 0, m0 = tile_m * S::ROWS_A, end = p.M, own_pair = 0;        // own_pair: of a quantising thread's row
   if (GROUPED) {
     pdl_wait();
-    if (warp == 0) {                                     // which expert's which rows: tiles of the experts, 32 at a time
+    if (FUSED && p.idx) {
+      // Few pairs: every CTA sorts them for itself (a launch less: 3 us).  Thread q counts the pairs of smaller experts, and those of its own in front
+      // of it; a tile begins at every ROWS_A-th row of an expert.  All of it lies where the ring will be.
+      int *expert = reinterpret_cast<int *>(smem), *rank_of = expert + MOST_INLINE, *begins = rank_of + MOST_INLINE, *pair_of = begins + MOST_INLINE;
+      const int q = threadIdx.x, n = p.M;
+      if (q < n) {
+        const int x = p.idx[q];
+        expert[q] = x >= 0 && x < p.n_experts ? x : p.n_experts;
+      }
+      if (q == 0) found[0] = -1;
+      __syncthreads();
+      int own = 0, first = 0, count = 0, rank = 0;
+      bool begin = false;
+      if (q < n) {
+        own = expert[q];
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+          const int x = expert[i];
+          first += x < own, count += x == own, rank += x == own && i < q;
+        }
+        begin = own < p.n_experts && rank % S::ROWS_A == 0;
+        rank += first;
+        rank_of[q] = rank, begins[q] = begin, pair_of[rank] = q;
+        if (p.pair_row && blockIdx.x == 0 && blockIdx.y == 0) p.pair_row[q] = own < p.n_experts ? rank : -1;
+      }
+      __syncthreads();
+      if (begin) {
+        int before = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) before += begins[i] && rank_of[i] < rank;
+        if (before == tile_m) found[0] = own, found[1] = rank, found[2] = first + count;
+      }
+      __syncthreads();
+      const int r = found[1] + ((int)threadIdx.x - (ADDERS + 2) * 32) / 8;
+      if (found[0] >= 0 && warp > ADDERS + 1 && r < found[2]) own_pair = pair_of[r];
+      fence_async_shared();                              // (in front of the copies that will be written there, and the barrier below)
+    } else if (warp == 0) {                              // which expert's which rows: tiles of the experts, 32 at a time
       int left = tile_m, at = -1, row = 0, last = 0;
       for (int e0 = 0; e0 < p.n_experts && at < 0; e0 += 32) {
         const int x = e0 + lane, first = x < p.n_experts ? p.starts[x] : 0, behind = x < p.n_experts ? p.starts[x + 1] : 0;
@@ -215,7 +251,8 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     // eight lanes a row, sixteen values each; AHEAD blocks are asked for before the first one is used
     const int r = (threadIdx.x - (ADDERS + 2) * 32) / 8, part = threadIdx.x % 8;
     const bool live = m0 + r < end;
-    const long long from = live ? (p.row_pair ? p.row_pair[m0 + r] / p.top : m0 + r) * p.x_stride : 0;
+    const int source = !live ? 0 : GROUPED && p.idx && p.gather ? own_pair / p.top : p.row_pair ? p.row_pair[m0 + r] / p.top : m0 + r;
+    const long long from = source * p.x_stride;
     const int n_block = min((GATED ? n0 / 2 : n0) / F8_BLOCK, p.nb - 1);
     const float *sw = p.sw + ((long long)e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks + kb0;
     bool ok = true;
@@ -496,7 +533,8 @@ static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few 
     if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A, FUSED>::SMEM, cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  const long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED>::ROWS_A + (GROUPED ? (p.M < p.n_experts ? p.M : p.n_experts) : 0);
+  long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED>::ROWS_A;
+  if (GROUPED) tiles_m = tiles_m + p.n_experts < p.M ? tiles_m + p.n_experts : p.M;       // (a tile has a row at least)
   const long long tiles_n = (p.N + Shape<NX, LANES_A, FUSED>::ROWS_W - 1) / Shape<NX, LANES_A, FUSED>::ROWS_W;
   if (tiles_n > 65535 || tiles_m * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
   g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, dim3((unsigned)(tiles_m * p.split), (unsigned)tiles_n), dim3(Shape<NX, LANES_A, FUSED>::THREADS),
@@ -506,7 +544,7 @@ static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few 
 
 template <int NX, bool LANES_A, bool FUSED>
 static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
-  if (p.starts) {
+  if (p.n_experts) {
     switch (epi) {
       case EPI_F32: return launch<NX, LANES_A, EPI_F32, true, FUSED>(map_a, map_w, p, stream);
       case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, true, FUSED>(map_a, map_w, p, stream);
@@ -519,7 +557,7 @@ static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, con
       case EPI_GATED_F32: return launch<NX, LANES_A, EPI_GATED_F32, false, FUSED>(map_a, map_w, p, stream);
     }
   }
-  G2B_REFUSE("gemm_fp8_few: no epilogue %d%s", epi, p.starts ? " for experts" : "");
+  G2B_REFUSE("gemm_fp8_few: no epilogue %d%s", epi, p.n_experts ? " for experts" : "");
 }
 
 // columns: 16, 32 or 64 rows of a side by side, or -64: 64 rows of w beside 128 of a; split: parts of K, at most 8.  With p.x (columns is 16 then): K a
@@ -527,6 +565,7 @@ static int pick(int epi, const CUtensorMap &map_a, const CUtensorMap &map_w, con
 static int run(const Product &given, int columns, int split, cudaStream_t stream) {
   if (given.x && (columns != 16 || given.K % 8 || given.x_stride % (given.x_f32 ? 4 : 8) || ((uintptr_t)given.x & 15) || given.top < 1))
     G2B_REFUSE("gemm_fp8_few: rows of %d values are not quantised on the way", given.K);
+  if (given.idx && (!given.x || given.M > MOST_INLINE || given.n_experts < 1)) G2B_REFUSE("gemm_fp8_few: %d pairs are not sorted by the product", given.M);
   if (split < 1 || split > MOST_SPLIT) G2B_REFUSE("gemm_fp8_few: %d parts of K", split);
   CUtensorMap map_a, map_w;
   int rc = get_map(&map_w, given.w, given.w_rows(), given.blocks * BK, (int)given.ldw, columns < 0 ? 64 : LANES, 1);

@@ -460,7 +460,7 @@ static int run(const Product &given, cudaStream_t stream) {
   Tc p;
   static_cast<Product &>(p) = given;
   p.nb = given.scale_rows();
-  if (given.starts) {
+  if (given.n_experts) {
     switch (given.epi) {
       case EPI_F32: return launch<EPI_F32, true>(map_a, map_w, p, stream);
       case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, true>(map_a, map_w, p, stream);
@@ -474,7 +474,7 @@ static int run(const Product &given, cudaStream_t stream) {
       case EPI_GATED_ROWS: return launch<EPI_GATED_ROWS, false>(map_a, map_w, p, stream);
     }
   }
-  G2B_REFUSE("gemm_fp8_tc: no epilogue %d%s", given.epi, given.starts ? " for experts" : "");
+  G2B_REFUSE("gemm_fp8_tc: no epilogue %d%s", given.epi, given.n_experts ? " for experts" : "");
 }
 
 }  // namespace many

@@ -95,7 +95,7 @@ static int check(const Product &p) {
   if (p.ldw % 16 || ((uintptr_t)p.w & 15) || (!p.x && (p.lda % 16 || ((uintptr_t)p.a & 15)))) G2B_REFUSE("products_fp8: rows must start on 16 bytes");
   if (p.gated() && p.N % 16) G2B_REFUSE("products_fp8: gates and ups in eights, got %d rows", p.N);
   if (p.epi == EPI_GATED_ROWS && (p.ldo % 16 || ((uintptr_t)p.out & 15))) G2B_REFUSE("products_fp8: quantised rows must start on 16 bytes");
-  if (p.starts && (p.n_experts < 1 || p.n_experts > MOST_EXPERTS)) G2B_REFUSE("products_fp8: %d experts outside 1..%d", p.n_experts, MOST_EXPERTS);
+  if (p.n_experts < 0 || p.n_experts > MOST_EXPERTS || (p.n_experts && !p.starts && !p.idx)) G2B_REFUSE("products_fp8: %d experts outside 1..%d", p.n_experts, MOST_EXPERTS);
   if (p.w_rows() > INT32_MAX || p.lda > INT32_MAX || p.ldw > INT32_MAX) G2B_REFUSE("products_fp8: %lld rows of W are too many", p.w_rows());
   return 0;
 }
@@ -202,15 +202,22 @@ extern "C" int g2b_fp8_experts(const Call *c, const void *h, const int *idx, uns
   d.w = w_down, d.sw = s_down, d.out = rows, d.ldo = c->H, d.N = c->H, d.K = inter, d.blocks = (inter + F8_BLOCK - 1) / F8_BLOCK, d.ldw = d.blocks * F8_BLOCK;
   d.epi = EPI_F32, d.top = 1;
   const Choice gated = c->first, down = c->second;
+  if (c->n_experts < 1) { snprintf(g2b_error_text, sizeof(g2b_error_text), "fp8_experts: %d experts", c->n_experts); return -1; }
   if (gated.with_x) {
     // few rows an expert: their places are enough, the products fetch and quantise them
     int *row_pair = reinterpret_cast<int *>(scratch);
     float *mid = reinterpret_cast<float *>(scratch + on_16((size_t)pairs * 4));
-    if (run_moe_sort(idx, pairs, c->n_experts, starts, pair_row, row_pair, stream)) return -1;
-    p.x = h, p.x_f32 = c->x_dtype == G2B_F32, p.x_stride = c->x_stride, p.row_pair = row_pair, p.out = mid, p.ldo = inter;
-    if (product(p, gated, stream)) return -1;
+    const bool inline_sort = pairs <= MOST_INLINE;
+    p.x = h, p.x_f32 = c->x_dtype == G2B_F32, p.x_stride = c->x_stride, p.out = mid, p.ldo = inter;
     d.x = mid, d.x_f32 = 1, d.x_stride = inter;
-    return product(d, down, stream) ? -1 : 3;
+    if (inline_sort) {
+      p.idx = d.idx = idx, p.starts = d.starts = nullptr, p.pair_row = pair_row, p.gather = 1;
+    } else {
+      if (run_moe_sort(idx, pairs, c->n_experts, starts, pair_row, row_pair, stream)) return -1;
+      p.row_pair = row_pair;
+    }
+    if (product(p, gated, stream)) return -1;
+    return product(d, down, stream) ? -1 : inline_sort ? 2 : 3;
   }
   const Rows sorted = rows_at(scratch, pairs, c->K), between = rows_at(scratch, pairs, inter);
   if (run_moe_sort(idx, pairs, c->n_experts, starts, pair_row, nullptr, stream)) return -1;

@@ -306,6 +306,40 @@ def test_experts(T, top, E, identity, I, K, hot):
     assert torch.equal(acc, base + out)
 
 
+@pytest.mark.parametrize("T,top,E,what", [(128, 1, 3, "one"), (43, 3, 5, "one"), (64, 2, 1024, "spread"), (33, 4, 200, "spread"), (40, 3, 7, "twice"),
+                                          (300, 3, 7, "twice"), (40, 2, 6, "nobody"), (400, 2, 6, "nobody"), (21, 6, 9, "outside"), (150, 6, 9, "outside")])
+def test_choices_of_every_kind(T, top, E, what):
+    """Few pairs, which the products sort by themselves, on both sides of their limit, and many: all of one expert, each of another, the same expert
+    twice in a token, numbers that no expert has.  Every row against the one that its expert alone gives its token."""
+    from gguf2bin_b200 import kernels, kernels_bf16
+    K, I = 256, 136
+    g = torch.Generator().manual_seed(T)
+    idx = {"one": torch.full((T, top), E - 1), "spread": torch.randint(0, E, (T, top), generator=g), "nobody": torch.full((T, top), E),
+           "twice": torch.randint(0, E, (T, 1), generator=g).expand(T, top),
+           "outside": torch.randint(-3, E + 3, (T, top), generator=g)}[what].to(torch.int32).contiguous().to(DEV)
+    x, _, weight, gu, down = experts_case(T, 1, E, 0, I, K, 3)
+    rows, pair_row = torch.full((T * top, K), 3.0, device=DEV), torch.full((T * top,), 77, dtype=torch.int32, device=DEV)
+    kernels.moe_experts_fp8(x, idx, gu, down, rows, pair_row)
+    kernels_bf16.check_status()
+    flat = idx.flatten().long()
+    real = (flat >= 0) & (flat < E)
+    order = torch.argsort(torch.where(real, flat, E), stable=True)[:int(real.sum())]
+    want = torch.full_like(pair_row, -1)
+    want[order] = torch.arange(len(order), dtype=torch.int32, device=DEV)
+    assert torch.equal(pair_row, want) and (rows[len(order):] == 3).all()
+    for e in flat[order].unique().tolist():
+        pairs = order[flat[order] == e]
+        one = torch.full((len(pairs), K), math.nan, device=DEV)
+        kernels.moe_experts_fp8(x[pairs // top].contiguous(), torch.zeros(len(pairs), 1, dtype=torch.int32, device=DEV),
+                                kernels.Fp8Matrix(gu.q[e:e + 1], gu.scale[e:e + 1], K), kernels.Fp8Matrix(down.q[e:e + 1], down.scale[e:e + 1], I), one,
+                                torch.empty(len(pairs), dtype=torch.int32, device=DEV))
+        got = rows[pair_row[pairs].long()]
+        # sums of K in other parts may move a value between over a border of e4m3: by a step, 2^-3 of it at most, were it all of them.  Another row's
+        # or expert's values are off by 2^0.5
+        assert (got - one).norm() <= 2.0 ** -3 * one.norm()
+    kernels_bf16.check_status()
+
+
 def test_a_feed_forward_on_another_stream_and_in_graphs():
     """Norm-sized rows -> gated product -> rows -> down product added to a stream: on a side stream, captured twice over one workspace, replayed in
     turn with new inputs; the bits of plain calls."""
@@ -389,9 +423,12 @@ def test_products_whose_copies_never_come(kernel):
     assert torch.equal(out, again) and out.abs().sum() > 0
 
 
-@pytest.mark.parametrize("columns", ["on the way", 16, 32, 64, -64])
-@pytest.mark.parametrize("split", [1, 2, 3, 4, 7, 8])
-@pytest.mark.parametrize("M,N,K", [(1, 130, 300), (13, 128, 1024), (40, 300, 2176), (150, 200, 640), (5, 64, 5000)])
+FEW = [(M, N, K, columns, split) for M, N, K in ((1, 130, 300), (13, 128, 1024), (40, 300, 2176), (150, 200, 640), (5, 64, 5000), (17, 72, 200))
+       for columns in ("on the way", 16, 32, 64, -64) for split in (1, 2, 3, 4, 7, 8)
+       if K % 8 == 0 or columns != "on the way"]         # (rows of other lengths are quantised first)
+
+
+@pytest.mark.parametrize("M,N,K,columns,split", FEW)
 def test_every_shape_of_few_rows(M, N, K, columns, split):
     """Each width and number of parts, ranges of K that are empty or of several chunks of scales, several tiles of rows."""
     from gguf2bin_b200 import kernels, kernels_bf16
@@ -401,8 +438,6 @@ def test_every_shape_of_few_rows(M, N, K, columns, split):
     a, m = rows_values(*rows), matrix_values(w.q, w.scale)
     out = torch.full((M, N), math.nan, device=DEV)
     fused = columns == "on the way"
-    if fused and K % 8:
-        pytest.skip("rows of values that are no multiple of eight are quantised first")
     K8._product("test", x if fused else rows, w, out, K8.EPI_F32, columns=K8.WITH_X if fused else columns, split=split)
     kernels_bf16.check_status()
     assert ((out.double() - a @ m.T).abs() <= (sum_bound(blocks_of(K)) + 8 * EPS) * (a.abs() @ m.abs().T) + 1e-44).all()
