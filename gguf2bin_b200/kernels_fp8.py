@@ -197,6 +197,12 @@ def gate_up_matrix(gate: Fp8Matrix, up: Fp8Matrix) -> Fp8Matrix:
     return Fp8Matrix(both.view(F8), torch.stack([gate.scale, up.scale]).contiguous(), gate.k)
 
 
+def no_matrix(n: int, k: int, device) -> Fp8Matrix:
+    """Zeros."""
+    return Fp8Matrix(torch.zeros((n, blocks_of(k) * BLOCK), dtype=torch.uint8, device=device).view(F8),
+                     torch.ones((blocks_of(n), blocks_of(k)), dtype=torch.float32, device=device), k)
+
+
 def stack_matrices(matrices) -> Fp8Matrix:
     """Matrices of one size as a stack (experts)."""
     q = torch.stack([m.q.view(torch.uint8) for m in matrices])

@@ -187,7 +187,7 @@ class GQAAttention:
         pad = -sum(p.shape[0] for p in parts) % 8 if self.wide else 0
         if self.eight_bit:
             if pad:
-                parts.append(kernels_fp8.quantize_matrix(torch.zeros((pad, self.hidden), device=parts[0].q.device)))
+                parts.append(kernels_fp8.no_matrix(pad, self.hidden, parts[0].q.device))
             self.w_qkv, self.w_o = kernels_fp8.side_by_side(parts), tensors[n["o"]]
         else:
             common = torch.float32 if any(p.dtype == torch.float32 for p in parts) else parts[0].dtype

@@ -90,3 +90,24 @@ def test_types_that_do_not_belong_are_one_error(tmp_path):
         load_weights(tmp_path, {"a": Expected((4, 4)), "b": Expected((4, 4), eight_bit=True), "b_scale_inv": Expected((1, 1))}, torch.bfloat16, "cpu")
     got = load_weights(tmp_path, {"a": Expected((4, 4), eight_bit=True), "b": Expected((4, 4)), "b_scale_inv": Expected((1, 1))}, torch.float32, "cpu")
     assert got["a"].dtype == torch.float8_e4m3fn and got["b"].dtype == torch.float32
+
+
+def test_a_mixer_binds_on_any_device():
+    """Head gates fill the rows up to a multiple of eight: no kernel may run for that (the model's device need not be the current one)."""
+    from mopitar_helpers import CONFIGS
+    from gguf2bin_b200.kernels import Fp8Matrices, Fp8Matrix
+    from gguf2bin_b200.parts.registry import mixer_class
+    from gguf2bin_b200.weights.eight_bit import F8
+    seen = 0
+    for cfg in CONFIGS.values():
+        spec = model_spec_from_dict(dict(cfg, quantization_config=FP8))
+        for layer in spec.layers:
+            if layer.mixer is None or not layer.mixer.get("eight_bit"):
+                continue
+            mixer = mixer_class(layer.mixer)(layer.mixer, spec.hidden_size, torch.float32, torch.device("cpu"))
+            expected = mixer_class(layer.mixer).expected(layer.mixer, spec.hidden_size)
+            mixer.bind({n: torch.ones(e.shape).to(F8) if e.eight_bit else torch.ones(e.shape) for n, e in expected.items()})
+            rows = sum(e.shape[0] for n, e in expected.items() if e.eight_bit) - expected[mixer.names["o"]].shape[0]
+            assert isinstance(mixer.w_qkv, (Fp8Matrix, Fp8Matrices)) and mixer.w_qkv.shape == (rows + -rows % 8, spec.hidden_size)
+            seen += rows % 8 != 0
+    assert seen
