@@ -115,6 +115,8 @@ def _check_rows(what: str, rows: Fp8Rows, k: int) -> None:
 def _check_matrix(what: str, w: Fp8Matrix, gated: bool, stacked: bool) -> None:
     q, s, k = w
     kb, lead = blocks_of(k), q.shape[:1] if stacked else ()
+    if k < 1:
+        raise KernelError(f"{what}: a matrix of {k} columns")
     if q.dtype != F8 or q.dim() != 2 + stacked or q.shape[-1] != kb * BLOCK or not q.is_contiguous() or q.data_ptr() % 16:
         raise KernelError(f"{what}: a matrix of {k} columns in 8 bits is contiguous float8_e4m3fn [{'experts, ' if stacked else ''}rows, "
                           f"{kb * BLOCK}] on 16 bytes; got {q.dtype} {list(q.shape)}")

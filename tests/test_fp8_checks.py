@@ -47,7 +47,7 @@ def test_products_are_checked():
                           (x, w, good.bfloat16(), dict(accumulate=True)), (x, w, torch.zeros(50, 3).t(), {}), (x, w._replace(k=100), good, {}),
                           (x, w._replace(scale=torch.zeros(2, 2)), good, {}), (x, w._replace(q=w.q.view(torch.uint8)), good, {}),
                           (x, w._replace(q=matrix(100, 200).q[::2]), good, {}), (rows(3, 300), w, good, {}), (rows(4, 200), w, good, {}),
-                          (x, matrix(50, 200, stack=2), good, {}), (x, w, torch.zeros(1, 50).expand(3, 50), {})):
+                          (x, matrix(50, 200, stack=2), good, {}), (torch.zeros(3, 0), matrix(50, 0), good, {}), (x, w, torch.zeros(1, 50).expand(3, 50), {})):
         with pytest.raises(KernelError):
             kernels.linear(a, m, out, **kw)
     for a in (x, rows(3, 200)):
