@@ -51,16 +51,17 @@ static double estimate(const Cost &k, long long tiles, int blocks, int split, in
 // The cheapest for activations that are still to be quantised; given rows go the same way, so that they have the same bits.  `experts`: the rows are
 // theirs, as many for each (those that have any), give or take.  rows_needed: quantised rows are to be left (only gemm_fp8_tc.cuh leaves them itself).
 static Choice choose(int M, int N, int blocks, int experts, bool rows_needed) {
-  const int used = experts ? (experts < M ? experts : M) : 1, each = (M + used - 1) / used;
+  const int used = experts ? (experts < M ? experts : M) : 1;
+  const long long each = ((long long)M + used - 1) / used;
   const double w_bytes = (double)used * N * blocks * F8_BLOCK;
   const double behind = rows_needed ? QUANTISED_FIRST + 1e-6 * M * N * 2.5 / 4 : 0;      // float, read and written again
-  const long long pairs_tiles = (long long)used * ((each + 255) / 256) * ((N + 255) / 256);
+  const long long pairs_tiles = used * ((each + 255) / 256) * ((N + 255) / 256);
   const int pairs = many::resident();
   Choice best = {0, 1, 0};
   double least = QUANTISED_FIRST + MANY_START + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * MANY_BLOCK + MANY_TILE);
   auto look = [&](int columns, bool x, const Cost &k, int (*resident)(int)) {
     const int rows_a = columns > 0 ? columns : 128, rows_w = columns > 0 ? 128 : 64;
-    const long long tiles = (long long)used * ((each + rows_a - 1) / rows_a) * ((N + rows_w - 1) / rows_w);
+    const long long tiles = used * ((each + rows_a - 1) / rows_a) * ((N + rows_w - 1) / rows_w);
     if (tiles > INT32_MAX / few::MOST_SPLIT) return;
     for (int split = 1; split <= few::MOST_SPLIT && split <= blocks; ++split) {
       const double us = estimate(k, tiles, blocks, split, resident(split), w_bytes) + (x ? 0 : QUANTISED_FIRST) + behind;
