@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from . import kernels
-from .kernels_bf16 import _status_word
+from .kernels_bf16 import _status, _status_word
 from .kernels import SILU, Fp8Matrices, Fp8Matrix, Fp8Rows, KernelError, _call, _code, _fn, _ptr, _stream
 
 ON_THE_WAY = 16                      # rows up to which a product quantises them itself (csrc/products_fp8.cu, choose)
@@ -51,6 +51,9 @@ def _f(name: str, argtypes, defines=()):
 
 
 def _plan(key, call: _Call, device, prepare: str, name: str, argtypes, x_aligned: bool, by_rule: bool = True, defines=()) -> _Plan:
+    if device not in _status and torch.cuda.is_current_stream_capturing():
+        # (the word that waits report to would be the graph's own memory, and gone with it)
+        raise KernelError(f"{name[4:]}: the first product on {device} cannot be captured; run it once before")
     plan = _Plan()
     plan.call, plan.at = call, addressof(call)
     size = _f(prepare, [c_void_p, c_int, c_int], defines)

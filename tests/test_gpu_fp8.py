@@ -385,6 +385,57 @@ def test_a_feed_forward_on_another_stream_and_in_graphs():
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+def test_the_first_product_is_not_captured(monkeypatch):
+    """The word that waits report to would be the graph's own memory: refused, and a later capture is what a call is."""
+    from gguf2bin_b200 import kernels, kernels_bf16
+    from gguf2bin_b200 import kernels_fp8 as K8
+    x, w = operands(20, 64, 256)
+    want, out = torch.empty(20, 64, device=DEV), torch.empty(20, 64, device=DEV)
+    kernels.linear(x, w, want)
+    word = dict(kernels_bf16._status)
+    K8._plans.clear()
+    kernels_bf16._status.clear()
+    try:
+        with pytest.raises(kernels.KernelError, match="captured"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                kernels.linear(x, w, out)
+    finally:
+        kernels_bf16._status.update(word)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kernels.linear(x, w, out)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    kernels_bf16.check_status()
+
+
+def test_two_streams_at_once():
+    """Products of every kernel and experts on two streams at the same time, without a workspace: each call has scratch memory of its own."""
+    from gguf2bin_b200 import kernels, kernels_bf16
+    cases = [operands(M, 512, 1000) for M in (3, 40, 200, 1500)]
+    h, idx, _, gu, down = experts_case(70, 3, 9, 0, 136, 256, 5)
+
+    def run():
+        outs = [torch.empty(len(x), 512, device=DEV) for x, _ in cases]
+        for (x, w), y in zip(cases, outs):
+            kernels.linear(x, w, y)
+        outs.append(torch.zeros(210, 256, device=DEV))
+        kernels.moe_experts_fp8(h, idx, gu, down, outs[-1], torch.empty(210, dtype=torch.int32, device=DEV))
+        return outs
+
+    want = run()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(run())
+    torch.cuda.synchronize()
+    kernels_bf16.check_status()
+    assert all(torch.equal(a, b) for outs in got for a, b in zip(outs, want))
+
+
 def test_empty_and_repeated_calls():
     from gguf2bin_b200 import kernels
     x, w = operands(0, 64, 64)
