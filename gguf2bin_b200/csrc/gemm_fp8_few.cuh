@@ -36,28 +36,31 @@ constexpr int most_sent(int columns, int unit) {
 }
 
 // LANES_A: the tile the other way round, 128 rows of A on the lanes of tensor memory and NX rows of W as its columns.
-// Two CTAs a multiprocessor.
-template <int NX, bool LANES_A, bool FUSED = false> struct Shape {
+// Two CTAs a multiprocessor; three with experts' rows in sixteens and half the ring, since an expert's tiles are many and short (64 tokens of 6 choices among 64
+// experts of 768 between 2,048: 82 us against 88, weights from DRAM).
+template <int NX, bool LANES_A, bool FUSED, bool GROUPED> struct Shape {
+  static constexpr bool MORE = GROUPED && !FUSED && NX == 16;
   static constexpr int ADD = NX >= 64 ? 2 : 1;           // groups of four adding warps
   static constexpr int COLS = NX / ADD;
-  static constexpr int STAGES = NX == 16 ? 6 : NX == 32 ? 5 : 4;
-  static constexpr int NACC = 4;                         // at most STAGES: a stage's barrier says both that its operands and that its sums are done
+  static constexpr int STAGES = MORE ? 3 : NX == 16 ? 6 : NX == 32 ? 5 : 4;
+  static constexpr int NACC = MORE ? 3 : 4;                       // at most STAGES: a stage's barrier says both that its operands and that its sums are done
   static constexpr int CHUNK = NX <= 32 ? 16 : 8;        // blocks whose scales are in shared memory at a time
   static constexpr int PITCH = LANES_A ? LANES + 1 : LANES;                           // of the columns sent: read along rows, or (LANES_A) along columns
   static constexpr int STAGE_BYTES = LANES * BK + NX * BK;
   static constexpr int RING = STAGES * STAGE_BYTES, SENT = most_sent(NX, LANES_A ? 16 : 4) / 4 * PITCH * 16;     // SENT lies where the ring was
   static constexpr int FACTORS = LANES_A ? 0 : 2 * CHUNK * NX * 4;
   static constexpr int SMEM = RING + FACTORS + 512 + 1024;                            // + barriers, + the swizzle's alignment
-  static constexpr int THREADS = (4 * ADD + 2 + (FUSED ? 4 : 0)) * 32, PER_SM = 2;
-  static constexpr int TMEM = NACC * NX;
+  static constexpr int THREADS = (4 * ADD + 2 + (FUSED ? 4 : 0)) * 32, PER_SM = MORE ? 3 : 2;
+  static constexpr int TMEM = 4 * NX;
   static constexpr int ROWS_A = LANES_A ? LANES : NX, ROWS_W = LANES_A ? NX : LANES;
   static_assert(!FUSED || (CHUNK > STAGES + NACC && NX == 16), "a block's scales stay until its sums are added");
+  static_assert((2 * STAGES + NACC + CHUNK) * 8 + (1 + 3 + MOST_INLINE) * 4 <= 512, "barriers and what a tile is found with");
   static_assert(NACC <= STAGES, "an adder must have seen a stage's barrier before its next products are issued");
   static_assert(SENT <= RING && PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * TMEM <= 512, "what a multiprocessor holds");
 };
 
 struct Few : Product {
-  int nb, split;                                         // nb: blocks of W's rows that have a scale
+  int nb, split, tiles_n;                                // nb: blocks of W's rows that have a scale
 };
 
 template <bool ACC>
@@ -95,9 +98,9 @@ __device__ __forceinline__ void got_columns(uint32_t (&x)[2][32]) {
 }
 
 template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
-__global__ void __launch_bounds__(Shape<NX, LANES_A, FUSED>::THREADS, Shape<NX, LANES_A, FUSED>::PER_SM)
+__global__ void __launch_bounds__(Shape<NX, LANES_A, FUSED, GROUPED>::THREADS, Shape<NX, LANES_A, FUSED, GROUPED>::PER_SM)
 gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ Few p) {
-  using S = Shape<NX, LANES_A, FUSED>;
+  using S = Shape<NX, LANES_A, FUSED, GROUPED>;
   constexpr bool GATED = EPI == EPI_GATED_F32;
   constexpr int ADDERS = 4 * S::ADD, CHUNK = S::CHUNK, PIECE = S::COLS < 32 ? S::COLS : 32, PIECES = S::COLS / PIECE;
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(LANES >> 4) << 24);      // accumulator float, operands e4m3, K-major
@@ -109,10 +112,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::RING + S::FACTORS);
   const uint32_t full0 = smem_addr(bars), done0 = full0 + 8 * S::STAGES, sum_empty0 = done0 + 8 * S::STAGES, scaled0 = sum_empty0 + 8 * S::NACC;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * S::STAGES + S::NACC + (FUSED ? CHUNK : 0));
-  int *found = reinterpret_cast<int *>(tmem_slot + 1);
+  int *found = reinterpret_cast<int *>(tmem_slot + 1), *pair_of = found + 3;              // pair_of: with p.idx, the pair of every row
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // (tiles of other rows of A, which read the same W, are neighbours)
-  const int rank = (int)(blockIdx.x % p.split), n0 = (int)blockIdx.y * S::ROWS_W, tile_m = (int)(blockIdx.x / p.split);
+  // Tiles of other rows of A, which read the same W, are neighbours.  Of experts, whose tiles along M are fewer than the grid's, those that are none come last.
+  const int rank = (int)(blockIdx.x % p.split), tile = (int)(blockIdx.x / p.split);
+  const int tile_m = GROUPED ? tile / p.tiles_n : tile, n0 = (GROUPED ? tile - tile_m * p.tiles_n : (int)blockIdx.y) * S::ROWS_W;
   const int per = (p.blocks + p.split - 1) / p.split, kb0 = rank * per, nkb = max(0, min(p.blocks, kb0 + per) - kb0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -124,45 +128,34 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       for (int b = 0; b < CHUNK; ++b) mbar_init(scaled0 + 8 * b, 4);
     mbar_init_fence();
   }
-  int e = 0, m0 = tile_m * S::ROWS_A, end = p.M, own_pair = 0;        // own_pair: of a quantising thread's row
+  int e = 0, m0 = tile_m * S::ROWS_A, end = p.M;
   if (GROUPED) {
     pdl_wait();
     if (FUSED && p.idx) {
-      // Few pairs: every CTA sorts them for itself (a launch less: 3 us).  Thread q counts the pairs of smaller experts, and those of its own in front
-      // of it; a tile begins at every ROWS_A-th row of an expert.  All of it lies where the ring will be.
-      int *expert = reinterpret_cast<int *>(smem), *rank_of = expert + MOST_INLINE, *begins = rank_of + MOST_INLINE, *pair_of = begins + MOST_INLINE;
-      const int q = threadIdx.x, n = p.M;
-      if (q < n) {
-        const int x = p.idx[q];
-        expert[q] = x >= 0 && x < p.n_experts ? x : p.n_experts;
-      }
-      if (q == 0) found[0] = -1;
-      __syncthreads();
-      int own = 0, first = 0, count = 0, rank = 0;
-      bool begin = false;
-      if (q < n) {
-        own = expert[q];
-#pragma unroll 4
+      // Few pairs: every CTA sorts them for itself, a pair a lane (a launch less: one token's four choices 32.5 -> 29.1 us).  A lane counts the pairs of
+      // smaller experts, and those of its own in front of it; a tile begins at every ROWS_A-th row of an expert.
+      if (warp == 0) {
+        const int n = p.M, x = lane < n ? p.idx[lane] : -1, own = x >= 0 && x < p.n_experts ? x : p.n_experts;
+        int first = 0, count = 0, row = 0, before = 0;
         for (int i = 0; i < n; ++i) {
-          const int x = expert[i];
-          first += x < own, count += x == own, rank += x == own && i < q;
+          const int y = __shfl_sync(0xffffffffu, own, i);
+          first += y < own, count += y == own, row += y == own && i < lane;
         }
-        begin = own < p.n_experts && rank % S::ROWS_A == 0;
-        rank += first;
-        rank_of[q] = rank, begins[q] = begin, pair_of[rank] = q;
-        if (p.pair_row && blockIdx.x == 0 && blockIdx.y == 0) p.pair_row[q] = own < p.n_experts ? rank : -1;
+        const bool begins = lane < n && own < p.n_experts && row % S::ROWS_A == 0;
+        const uint32_t all = __ballot_sync(0xffffffffu, begins);
+        row += first;
+        for (int i = 0; i < n; ++i) {
+          const int y = __shfl_sync(0xffffffffu, row, i);
+          before += (all >> i & 1) && y < row;
+        }
+        const bool hit = begins && before == tile_m;
+        if (hit) found[0] = own, found[1] = row, found[2] = first + count;
+        if (!__any_sync(0xffffffffu, hit) && lane == 0) found[0] = -1;
+        if (lane < n) {
+          pair_of[row] = lane;
+          if (p.pair_row && blockIdx.x == 0) p.pair_row[lane] = own < p.n_experts ? row : -1;
+        }
       }
-      __syncthreads();
-      if (begin) {
-        int before = 0;
-#pragma unroll 4
-        for (int i = 0; i < n; ++i) before += begins[i] && rank_of[i] < rank;
-        if (before == tile_m) found[0] = own, found[1] = rank, found[2] = first + count;
-      }
-      __syncthreads();
-      const int r = found[1] + ((int)threadIdx.x - (ADDERS + 2) * 32) / 8;
-      if (found[0] >= 0 && warp > ADDERS + 1 && r < found[2]) own_pair = pair_of[r];
-      fence_async_shared();                              // (in front of the copies that will be written there, and the barrier below)
     } else if (warp == 0) {                              // which expert's which rows: tiles of the experts, 32 at a time
       int left = tile_m, at = -1, row = 0, last = 0;
       for (int e0 = 0; e0 < p.n_experts && at < 0; e0 += 32) {
@@ -251,7 +244,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     // eight lanes a row, sixteen values each; AHEAD blocks are asked for before the first one is used
     const int r = (threadIdx.x - (ADDERS + 2) * 32) / 8, part = threadIdx.x % 8;
     const bool live = m0 + r < end;
-    const int source = !live ? 0 : GROUPED && p.idx && p.gather ? own_pair / p.top : p.row_pair ? p.row_pair[m0 + r] / p.top : m0 + r;
+    const int source = !live ? 0 : GROUPED && p.idx && p.gather ? pair_of[m0 + r] / p.top : p.row_pair ? p.row_pair[m0 + r] / p.top : m0 + r;
     const long long from = source * p.x_stride;
     const int n_block = min((GATED ? n0 / 2 : n0) / F8_BLOCK, p.nb - 1);
     const float *sw = p.sw + ((long long)e * (GATED ? 2 : 1) * p.nb + n_block) * p.blocks + kb0;
@@ -376,7 +369,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
       if (!ok) continue;
       tc_fence_after();
       const float *f = mine + i % CHUNK * NX;
-uint32_t x[PIECES][PIECE];
+      uint32_t x[PIECES][PIECE];
       ask_columns(from0 + h * NX, x);
       got_columns(x);
       tc_fence_before();
@@ -495,29 +488,29 @@ uint32_t x[PIECES][PIECE];
 
 template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
 static cudaError_t allow() {
-  return cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX, LANES_A, FUSED>::SMEM);
+  return cudaFuncSetAttribute(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<NX, LANES_A, FUSED, GROUPED>::SMEM);
 }
 
-// How many CTAs in clusters of `split` the device holds at once.  The runtime counts one CTA a multiprocessor for a kernel that allocates tensor memory; two
-// are there (148 tiles 4.6 us, 296 5.8, 444 9.6).
-template <int NX, bool LANES_A, bool FUSED>
+// How many CTAs in clusters of `split` the device holds at once.  The runtime counts one CTA a multiprocessor for a kernel that allocates tensor memory; there are
+// PER_SM (two: 148 tiles 4.6 us, 296 5.8, 444 9.6).
+template <int NX, bool LANES_A, bool FUSED, bool GROUPED>
 static int resident(int split) {
   static G2bPerDevice kept[MOST_SPLIT + 1];
   const int dev = g2b_current_device();
   if (dev >= 0 && kept[split].value[dev] > 0) return kept[split].value[dev];
   int clusters = 0, each = 0;
-  if (allow<NX, LANES_A, EPI_F32, false, FUSED>() == cudaSuccess) {
+  if (allow<NX, LANES_A, EPI_F32, GROUPED, FUSED>() == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split), cfg.blockDim = dim3(Shape<NX, LANES_A, FUSED>::THREADS), cfg.dynamicSmemBytes = Shape<NX, LANES_A, FUSED>::SMEM;
+    cfg.gridDim = dim3(split), cfg.blockDim = dim3(Shape<NX, LANES_A, FUSED, GROUPED>::THREADS), cfg.dynamicSmemBytes = Shape<NX, LANES_A, FUSED, GROUPED>::SMEM;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = split, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr, cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&clusters, gemm_fp8_few_kernel<NX, LANES_A, EPI_F32, false, FUSED>, &cfg) != cudaSuccess) clusters = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, gemm_fp8_few_kernel<NX, LANES_A, EPI_F32, false, FUSED>, Shape<NX, LANES_A, FUSED>::THREADS,
-                                                      Shape<NX, LANES_A, FUSED>::SMEM) != cudaSuccess)
+    if (cudaOccupancyMaxActiveClusters(&clusters, gemm_fp8_few_kernel<NX, LANES_A, EPI_F32, GROUPED, FUSED>, &cfg) != cudaSuccess) clusters = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&each, gemm_fp8_few_kernel<NX, LANES_A, EPI_F32, GROUPED, FUSED>, Shape<NX, LANES_A, FUSED, GROUPED>::THREADS,
+                                                      Shape<NX, LANES_A, FUSED, GROUPED>::SMEM) != cudaSuccess)
       each = 0;
-    if (each == 1) clusters *= Shape<NX, LANES_A, FUSED>::PER_SM;
+    if (each == 1) clusters *= Shape<NX, LANES_A, FUSED, GROUPED>::PER_SM;
   }
   const int n = clusters > 0 ? clusters * split : 1;
   if (dev >= 0) kept[split].value[dev] = n;
@@ -525,20 +518,22 @@ static int resident(int split) {
 }
 
 template <int NX, bool LANES_A, int EPI, bool GROUPED, bool FUSED>
-static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, const Few &p, cudaStream_t stream) {
+static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, Few p, cudaStream_t stream) {
   static G2bPerDevice configured;
   const int dev = g2b_current_device();
   if (dev < 0 || !configured.value[dev]) {
     const cudaError_t e = allow<NX, LANES_A, EPI, GROUPED, FUSED>();
-    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A, FUSED>::SMEM, cudaGetErrorString(e));
+    if (e != cudaSuccess) G2B_REFUSE("gemm_fp8_few: %d bytes of shared memory: %s", Shape<NX, LANES_A, FUSED, GROUPED>::SMEM, cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }
-  long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED>::ROWS_A;
+  long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_A;
   if (GROUPED) tiles_m = tiles_m + p.n_experts < p.M ? tiles_m + p.n_experts : p.M;       // (a tile has a row at least)
-  const long long tiles_n = (p.N + Shape<NX, LANES_A, FUSED>::ROWS_W - 1) / Shape<NX, LANES_A, FUSED>::ROWS_W;
-  if (tiles_n > 65535 || tiles_m * p.split > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
-  g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, dim3((unsigned)(tiles_m * p.split), (unsigned)tiles_n), dim3(Shape<NX, LANES_A, FUSED>::THREADS),
-                     (size_t)Shape<NX, LANES_A, FUSED>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
+  const long long tiles_n = (p.N + Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_W - 1) / Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_W;
+  if ((!GROUPED && tiles_n > 65535) || tiles_m * p.split * (GROUPED ? tiles_n : 1) > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
+  p.tiles_n = (int)tiles_n;
+  const dim3 grid((unsigned)(tiles_m * p.split * (GROUPED ? tiles_n : 1)), GROUPED ? 1u : (unsigned)tiles_n);
+  g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, grid, dim3(Shape<NX, LANES_A, FUSED, GROUPED>::THREADS),
+                     (size_t)Shape<NX, LANES_A, FUSED, GROUPED>::SMEM, stream, (unsigned)p.split, map_a, map_w, p);
   return g2b_check_launch("gemm_fp8_few");
 }
 

@@ -306,8 +306,9 @@ def test_experts(T, top, E, identity, I, K, hot):
     assert torch.equal(acc, base + out)
 
 
-@pytest.mark.parametrize("T,top,E,what", [(128, 1, 3, "one"), (43, 3, 5, "one"), (64, 2, 1024, "spread"), (33, 4, 200, "spread"), (40, 3, 7, "twice"),
-                                          (300, 3, 7, "twice"), (40, 2, 6, "nobody"), (400, 2, 6, "nobody"), (21, 6, 9, "outside"), (150, 6, 9, "outside")])
+@pytest.mark.parametrize("T,top,E,what", [(32, 1, 3, "one"), (11, 3, 5, "one"), (128, 1, 3, "one"), (16, 2, 1024, "spread"), (64, 2, 1024, "spread"),
+                                          (33, 4, 200, "spread"), (10, 3, 7, "twice"), (40, 3, 7, "twice"), (300, 3, 7, "twice"), (9, 2, 6, "nobody"),
+                                          (40, 2, 6, "nobody"), (400, 2, 6, "nobody"), (5, 6, 9, "outside"), (21, 6, 9, "outside"), (150, 6, 9, "outside")])
 def test_choices_of_every_kind(T, top, E, what):
     """Few pairs, which the products sort by themselves, on both sides of their limit, and many: all of one expert, each of another, the same expert
     twice in a token, numbers that no expert has.  Every row against the one that its expert alone gives its token."""
