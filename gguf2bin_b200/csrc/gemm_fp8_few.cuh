@@ -16,6 +16,12 @@
 // `starts`: W is a stack of matrices and rows starts[e] .. starts[e + 1] of A meet the e-th.  Gated: rows of W alternate, eight gates and the eight
 // ups of the same outputs, each with the scales of their own matrix.
 //
+// What bounds it: W's bytes where there are enough of them, else the way of a block of K: copy, four products and a commit (0.24 us of issue, whatever N
+// is and wherever W lies), tensor memory, sums.  Hence K in parts where tiles are few (each part more costs 0.6 us and its exchange), two CTAs a
+// multiprocessor, so that one's issue hides the other's, and 128 rows of A on the lanes from some 70 rows on (no factors from shared memory, 64 rows of W a
+// tile).  Measured, products behind one another in a graph, quantising included: 1 row by 6,144 x 4,096 6.8 us (25 MB), 8 rows' gate and up of 12,288 x 4,096
+// 18.4 (5.5 TB/s; a copy reaches 6.45), 64 by 5,120 x 17,408 18.2 with given rows (4.9 TB/s), 128 by 6,144 x 4,096 11.1, 256 by 4,096 x 4,096 10.9.
+//
 // Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
 #pragma once
 #include "product_fp8.cuh"

@@ -14,6 +14,12 @@
 // ups of the same outputs, each with the scales of their own matrix; a tile is then 128 outputs wide, one block of the rows that the next product
 // reads, so their scale is known where they are made.
 //
+// What bounds it: the sums' way out of tensor memory beside the products.  A block of K is 512 cycles of products and takes about 900 of the adders' round of
+// waiting, loading and adding; the tensor pipe is busy 56 % of the time (8,192 rows by 4,096 x 12,288), DRAM 21 %, the issue slots 38 %.  Without the
+// additions a block takes 640 to 690 cycles, and more of an accumulator on its way at once makes it longer (four pieces, or the next block's first ones
+// behind this one's last: 3 to 8 % slower).  The walk over all of it then meets the power cap: 2,048 rows by 6,144 x 4,096 50 us cool and 55 hot (2,060 and
+// 1,870 TFLOP/s), 8,192 by 4,096 x 12,288 added to a stream 382 and 441, gate and up of 17,408 x 5,120 at 2,048 rows 316 and 370 (2,310 and 1,970).
+//
 // Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
 #pragma once
 #include "product_fp8.cuh"

