@@ -333,14 +333,16 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       }
       if (rows <= 0) continue;
       // 32 rows of 128 bytes at a time through a box: written out (or added to what is there: every output gets one addition) by the copy unit,
-      // or, where C's rows do not start on 16 bytes or some of the rows are another expert's, read back by the warp, eight lanes a row.
+      // or, where C's rows do not start on 16 bytes or some of the rows are another expert's, read back by the warp.
       constexpr int OUTS = GATED ? COLS / 2 : COLS, WIDE = EPI == EPI_BF16 ? 64 : 32;
       const int n_out = GATED ? p.N / 2 : p.N, first = GATED ? (n0 + col0) / 2 : n0 + col0;
-      const bool copied = p.boxes && (!GROUPED || rows == 32);
+      // (the copy unit cuts a row off at 16 bytes only: what lies behind C's last column may be another's)
+      const bool cut = n_out % (EPI == EPI_BF16 ? 8 : 4) != 0;
 #pragma unroll
       for (int q = 0; q < OUTS / WIDE; ++q) {
         const int n1 = first + WIDE * q;
         if (n1 >= n_out) break;
+        const bool copied = p.boxes && (!GROUPED || rows == 32) && !(cut && n1 + WIDE > n_out);
         int l = lane;
         asm volatile("" : "+r"(l));                      // or the boxes' addresses are kept over the loop above
         unsigned char *const at = boxes + box * BOX_BYTES;
@@ -372,27 +374,37 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             else tma_store_2d(&map_out, smem_addr(at), n1, m0);
             bulk_commit();
           }
-        } else {
+        } else if (p.boxes && n1 + WIDE <= n_out) {      // (of an expert's last rows; nothing is added to there)
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const int r = 4 * i + lane / 8, j = lane % 8, n = n1 + WIDE / 8 * j;
+            const int r = 4 * i + lane / 8, j = lane % 8;
             if (r >= rows) break;
-            const uint4 w = *reinterpret_cast<const uint4 *>(at + r * 128 + ((j ^ (r & 7)) << 4));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-            const long long to = (long long)(m0 + r) * p.ldo + n;
-            if (p.boxes && n + WIDE / 8 <= n_out) {      // (of an expert's last rows; nothing is added to there)
-              *reinterpret_cast<uint4 *>(static_cast<unsigned char *>(p.out) + to * (EPI == EPI_BF16 ? 2 : 4)) = w;
-              continue;
-            }
+            *reinterpret_cast<uint4 *>(static_cast<unsigned char *>(p.out) + ((long long)(m0 + r) * p.ldo + n1 + WIDE / 8 * j) * (EPI == EPI_BF16 ? 2 : 4)) =
+                *reinterpret_cast<const uint4 *>(at + r * 128 + ((j ^ (r & 7)) << 4));
+          }
+          __syncwarp();
+        } else {
+          // rows that start anywhere: neighbouring lanes neighbouring outputs of a row (four a lane: 2,115 rows by 7,079 x 4,046 into a stream 218 us)
+          if (lane == 0) bulk_commit();                  // (nothing: boxes are counted by their groups)
+          __syncwarp();
+          constexpr int SIZE = EPI == EPI_BF16 ? 2 : 4, EACH = 16 / SIZE, ROWS = 8;
 #pragma unroll
-            for (int e = 0; e < WIDE / 8; ++e) {
-              if (n + e >= n_out) break;
-              if (EPI == EPI_BF16) {
-                static_cast<uint16_t *>(p.out)[to + e] = (uint16_t)(u[e / 2] >> 16 * (e & 1));
-              } else {
-                float *one = static_cast<float *>(p.out) + to + e;
-                *one = EPI == EPI_ADD_F32 ? *one + __uint_as_float(u[e]) : __uint_as_float(u[e]);
+          for (int c = lane; c < WIDE; c += 32) {
+            if (n1 + c >= n_out) break;
+            unsigned char *to = static_cast<unsigned char *>(p.out) + ((long long)m0 * p.ldo + n1 + c) * SIZE;
+            for (int r0 = 0; r0 < rows; r0 += ROWS) {
+              float old[ROWS];
+#pragma unroll
+              for (int i = 0; i < ROWS; ++i) old[i] = EPI == EPI_ADD_F32 && r0 + i < rows ? *reinterpret_cast<const float *>(to + (r0 + i) * p.ldo * SIZE) : 0.f;
+#pragma unroll
+              for (int i = 0; i < ROWS; ++i) {
+                const int r = r0 + i;
+                if (r >= rows) break;
+                const unsigned char *v = at + r * 128 + ((c / EACH ^ (r & 7)) << 4) + c % EACH * SIZE;
+                if (EPI == EPI_BF16) *reinterpret_cast<uint16_t *>(to + r * p.ldo * SIZE) = *reinterpret_cast<const uint16_t *>(v);
+                else if (EPI == EPI_ADD_F32) *reinterpret_cast<float *>(to + r * p.ldo * SIZE) = old[i] + *reinterpret_cast<const float *>(v);
+                else *reinterpret_cast<float *>(to + r * p.ldo * SIZE) = *reinterpret_cast<const float *>(v);
               }
             }
           }

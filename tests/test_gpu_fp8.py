@@ -134,6 +134,33 @@ def test_products(M, N, K):
     kernels_bf16.check_status()
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 8, 130), (100, 257, 300), (300, 1000, 640), (530, 1537, 200)])
+def test_many_rows_stored_anywhere(M, N, K):
+    """The kernel of many rows, whatever the sizes would choose: outputs on 16 bytes and at odd places and strides, nothing written beside them."""
+    from gguf2bin_b200 import kernels_bf16
+    from gguf2bin_b200 import kernels_fp8 as K8
+    from gguf2bin_b200.kernels import Fp8Rows
+    x, w = operands(M, N, K)
+    rows = Fp8Rows(*held(x))
+    a, m = rows_values(*rows), matrix_values(w.q, w.scale)
+    ref, bound = a @ m.T, sum_bound(blocks_of(K)) * (a.abs() @ m.abs().T) + 1e-44
+    base, first = rnd(M, N, seed=2), None
+    for before, behind in ((0, -N % 8), (1, 2), (3, 4), (8, 8 - N % 8)):
+        at = slice(before, before + N)
+        out, acc = torch.full((M, before + N + behind), 7.0, device=DEV), torch.full((M, before + N + behind), 7.0, device=DEV)
+        half = torch.full((M, before + N + behind), 7.0, dtype=torch.bfloat16, device=DEV)
+        acc[:, at] = base
+        K8._product("test", rows, w, out[:, at], K8.EPI_F32, columns=0)
+        K8._product("test", rows, w, acc[:, at], K8.EPI_ADD_F32, columns=0)
+        K8._product("test", rows, w, half[:, at], K8.EPI_BF16, columns=0)
+        kernels_bf16.check_status()
+        first = out[:, at].clone() if first is None else first
+        assert ((first.double() - ref).abs() <= bound).all() and torch.equal(out[:, at], first)
+        assert torch.equal(acc[:, at], base + first) and torch.equal(half[:, at], first.to(torch.bfloat16))
+        for t in (out, acc, half):
+            assert (t[:, :before] == 7).all() and (t[:, before + N:] == 7).all()
+
+
 def test_products_of_odd_rows():
     """Rows with infinities and NaN are NaN, rows of zeros zeros, and the others have the bits that they have alone."""
     from gguf2bin_b200 import kernels
