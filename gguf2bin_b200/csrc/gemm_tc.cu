@@ -1508,8 +1508,10 @@ static int make_map(CUtensorMap *map, const void *base, int rows, int K, int ld,
   return 0;
 }
 
-// A map of C for the tile stores of the persistent kernel: boxes of 32 rows x 128 bytes.
+// A map of C for the tile stores of the persistent kernel: boxes of 32 rows x 128 bytes.  The copy unit cuts a row off at 16 bytes only: it
+// would write zeros behind a last column that ends between them.
 static int make_map_c(CUtensorMap *map, const void *base, int rows, int cols, int ld, bool is_float) {
+  if (cols * (is_float ? 4ll : 2ll) % 16) G2B_REFUSE("gemm_tc: tile stores end on 16 bytes, not behind %d columns", cols);
   const int rc = get_map(map, base, rows, cols, ld, 32, is_float ? 4 : 2);
   if (rc) G2B_REFUSE("gemm_tc: cuTensorMapEncodeTiled for C failed or is not available (code %d)", rc);
   return 0;

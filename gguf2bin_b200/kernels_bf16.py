@@ -176,7 +176,7 @@ def _route(a: torch.Tensor, w: torch.Tensor, out: torch.Tensor):
     """Which kernel multiplies a by w.T into out, and with which tile shape: decided once per
     combination of sizes, strides and alignments (a step asks the same few questions a hundred
     times, and on a prompt's first run the host is what the GPU waits for)."""
-    key = (a.shape, w.shape, a.stride(), w.stride(), out.stride(), out.dtype,
+    key = (a.shape, w.shape, a.stride(), w.stride(), out.shape, out.stride(), out.dtype,
            (a.data_ptr() | w.data_ptr()) & 15, out.data_ptr() & 15, out.device.index)
     r = _routes.get(key)
     if r is None:
@@ -351,7 +351,8 @@ def _normed_loses(M: int, N: int, K: int) -> bool:
 def _tc_shape(M: int, N: int, out: torch.Tensor = None, K: int = 0):
     """(tile width, stages, persistent) of the tcgen05 product; (0, 0, False) lets the launcher
     choose.  Prompts (more than one row of tiles) take the persistent kernel when C can be
-    written as tiles (the launcher picks the tile width, and with few tiles K in parts); long prompts
+    written as tiles (the launcher picks the tile width, and with few tiles K in parts; the copy unit cuts a row off at 16 bytes
+only, so C is not where its columns end between them: zeros would be written behind the last one); long prompts
     take pairs of CTAs (persistent = 2; measured 4-9 % faster from 4,096 rows on, the same or
     slower at 2,048 with the short K of a small model; with a K of 4,096 and more from 1,024 rows on)."""
     if M <= 128:                       # one row of tiles: the weights stream, as in decode
@@ -359,7 +360,8 @@ def _tc_shape(M: int, N: int, out: torch.Tensor = None, K: int = 0):
             return (0, 0, 3)           # 128 rows of W per CTA, K split over a cluster
         if not (M > 64 and N >= 2048 and K >= 2048 and N <= 65536):      # (else the persistent kernel, below)
             return (128, 3, False) if N >= 32768 else (64, 8, False)
-    if out is not None and out.data_ptr() % 16 == 0 and (out.stride(0) * out.element_size()) % 16 == 0:
+    if out is not None and out.data_ptr() % 16 == 0 and (out.stride(0) * out.element_size()) % 16 == 0 and \
+            (out.shape[-1] * out.element_size()) % 16 == 0:
         tiles = -(-M // 256) * -(-N // 256)
         if M >= 4096 and tiles >= _sm_count(out.device) // 2:
             return (256, 6, 2)               # long prompts: pairs of CTAs on 256 x 256 tiles
