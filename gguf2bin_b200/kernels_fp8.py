@@ -104,7 +104,7 @@ def _on_device(what: str, *tensors) -> None:
         raise KernelError(f"{what}: tensors on the devices {sorted(set(at))}, while the current device is {here}")
 
 
-def _check_rows(what: str, rows: Fp8Rows, k: int) -> None:
+def _check_rows(what: str, rows: Fp8Rows, k: int, written: bool = False) -> None:
     q, s = rows
     kb = blocks_of(k)
     if q.dtype != F8 or q.dim() != 2 or q.shape[1] != kb * BLOCK or q.stride(1) != 1 or q.stride(0) % 16 or q.data_ptr() % 16 or \
@@ -113,6 +113,8 @@ def _check_rows(what: str, rows: Fp8Rows, k: int) -> None:
                           f"{q.dtype} {list(q.shape)} with strides {list(q.stride())}")
     if s.dtype != torch.float32 or tuple(s.shape) != (kb, q.shape[0]) or (s.shape[1] > 1 and s.stride(1) != 1):
         raise KernelError(f"{what}: the rows' scales are float32 [{kb}, {q.shape[0]}], rows innermost; got {s.dtype} {list(s.shape)}")
+    if written and kb > 1 and s.stride(0) < s.shape[1]:
+        raise KernelError(f"{what}: the rows' scales that are written do not overlap; got {list(s.shape)} with strides {list(s.stride())}")
 
 
 def _check_matrix(what: str, w: Fp8Matrix, gated: bool, stacked: bool) -> None:
@@ -152,7 +154,7 @@ def _plan_rows(key, x, rows: Fp8Rows, pair_row) -> tuple:
     tokens, k = x.shape
     if k < 1:
         raise KernelError("quantize_rows: rows without values")
-    _check_rows("quantize_rows", rows, k)
+    _check_rows("quantize_rows", rows, k, written=True)
     top = 1
     if pair_row is not None:
         top = pair_row.numel() // max(tokens, 1)
@@ -245,7 +247,7 @@ def _plan_product(key, what: str, a, w: Fp8Matrix, out, epi: int, form, columns:
     tokens = (a.q if given else a).shape[0]
     n = w.q.shape[0] // 2 if gated else w.q.shape[0]
     if as_rows:
-        _check_rows(what, out, n)
+        _check_rows(what, out, n, written=True)
         if out.q.shape[0] != tokens:
             raise KernelError(f"{what}: {tokens} rows into {out.q.shape[0]}")
     else:
