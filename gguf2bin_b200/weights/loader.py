@@ -93,6 +93,8 @@ def load_weights(folder, expected: Mapping[str, Expected], compute_dtype: torch.
         check_names_and_shapes(expected, {n: f.entries[n].shape for n, f in where.items()})
         odd = [f"    {n}  has unsupported dtype {f.entries[n].dtype}, expected {'F8_E4M3' if expected[n].eight_bit else 'one of more than 8 bits'}"
                for n, f in where.items() if (f.entries[n].dtype == "F8_E4M3") != expected[n].eight_bit]
+        odd += [f"    {n}  has unsupported dtype {f.entries[n].dtype}, expected F32, F64, BF16 or F16 for blocks' scales"
+                for n, f in where.items() if expected[n].init == "block_scales" and f.entries[n].dtype not in ("F32", "F64", "BF16", "F16", "F8_E4M3")]
         if odd:
             raise WeightsError("\n".join([f"weights do not match the model:\n  wrong type ({len(odd)}), by quantization_config of config.json:"] + odd))
         out = {}
@@ -100,7 +102,9 @@ def load_weights(folder, expected: Mapping[str, Expected], compute_dtype: torch.
             if name not in where:
                 continue
             cpu = where[name].tensor(name)
-            kept = cpu.dtype if expected[name].eight_bit else runtime_dtype(cpu.dtype, compute_dtype)
+            e = expected[name]
+            # (a scale is a factor of a whole block: it is 32 bits wide, whatever the model computes in)
+            kept = cpu.dtype if e.eight_bit else torch.float32 if e.init == "block_scales" else runtime_dtype(cpu.dtype, compute_dtype)
             out[name] = cpu.to(device=device, dtype=kept, copy=True)
             del cpu
         return out
