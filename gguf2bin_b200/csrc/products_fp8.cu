@@ -175,7 +175,7 @@ extern "C" long long g2b_fp8_experts_plan(Call *c, int x_aligned, int by_rule) {
   const long long pairs = (long long)c->M * c->top;
   const int inter = c->N / 2, blocks = (c->K + F8_BLOCK - 1) / F8_BLOCK, blocks_down = (inter + F8_BLOCK - 1) / F8_BLOCK;
   size_t bytes = on_16((size_t)(c->n_experts + 1) * 4);
-  if (pairs > INT32_MAX) return (long long)bytes;        // (the call refuses it)
+  if (pairs <= 0 || pairs > INT32_MAX) return (long long)bytes;        // (the call has nothing to do, or refuses it)
   if (by_rule) {
     // both products quantise their rows, or neither does; where both do, few pairs need no kernel that sorts them (4 tokens of 6 choices among 64 experts of
     // 768 between 2,048: 22.2 us against 25.0; 16 tokens, sorted first: 52 against 47)
