@@ -92,10 +92,11 @@ static void launch_rows(int vec, dim3 grid, cudaStream_t stream, const void *x, 
              blocks, (uint8_t *)q, q_stride, scale, scale_stride, pair_row, top, n_rows);
 }
 
-// pair_row: int [tokens * top], or null (then every row of x has a row of q); places outside 0 .. n_rows - 1 are left out.  q's rows on 16 bytes.
+// pair_row: int [tokens * top], or null (then every row of x has a row of q, and top is 1); places outside 0 .. n_rows - 1 are left out.  No choices
+// (top 0, whose places have no address either): nothing is written.  q's rows on 16 bytes.
 static int run_quantize_rows(const void *x, int dtype, long long x_stride, int tokens, int K, void *q, long long q_stride, float *scale,
                                  long long scale_stride, const int *pair_row, int top, int n_rows, cudaStream_t stream) {
-  if (tokens <= 0 || K <= 0) return 0;
+  if (tokens <= 0 || K <= 0 || top <= 0) return 0;
   const int blocks = (K + F8_BLOCK - 1) / F8_BLOCK;
   if (q_stride % 16 || q_stride < (long long)blocks * F8_BLOCK || ((uintptr_t)q & 15))
     G2B_REFUSE("quantize_rows: rows of q start on 16 bytes and hold %d blocks of %d", blocks, F8_BLOCK);

@@ -52,3 +52,11 @@ def test_experts_of_no_pairs(tokens, top, dtype):
     kernels.quantize_rows(x, kernels.Fp8Rows(q.q[:0], q.scale[:, :0]), ints(tokens, 0))
     kernels_bf16.check_status()
     torch.cuda.synchronize()
+
+
+def test_rows_without_places_are_written_nowhere():
+    """Places [T, 0] have no address: nothing is launched for them (here, without a device, a launch is an error)."""
+    from ctypes import c_int, c_longlong, c_void_p
+    from gguf2bin_b200 import kernels_fp8 as K8
+    f = K8._f("g2b_quantize_rows", [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p])
+    assert f(None, 0, 256, 5, 256, None, 256, None, 0, None, 0, 0, None) == 0
