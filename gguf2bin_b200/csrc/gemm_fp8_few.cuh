@@ -32,6 +32,7 @@ constexpr int LANES = 128, BK = F8_BLOCK, LANE_BYTES = LANES * BK;
 enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
 
 constexpr int MOST_SPLIT = 8;
+constexpr int MOST_TILES_N = 65535;                      // a product's tiles along W's rows are the grid's second axis
 // columns that a CTA of `split` owns, `unit` at a time, and the most that ranges and columns owned come to
 constexpr int columns_owned(int columns, int unit, int split) { return (columns / unit + split - 1) / split * unit; }
 constexpr int most_sent(int columns, int unit) {
@@ -555,7 +556,7 @@ static int launch(const CUtensorMap &map_a, const CUtensorMap &map_w, Few p, cud
   long long tiles_m = ((long long)p.M + Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_A - 1) / Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_A;
   if (GROUPED) tiles_m = tiles_m + p.n_experts < p.M ? tiles_m + p.n_experts : p.M;       // (a tile has a row at least)
   const long long tiles_n = (p.N + Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_W - 1) / Shape<NX, LANES_A, FUSED, GROUPED>::ROWS_W;
-  if ((!GROUPED && tiles_n > 65535) || tiles_m * p.split * (GROUPED ? tiles_n : 1) > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
+  if ((!GROUPED && tiles_n > MOST_TILES_N) || tiles_m * p.split * (GROUPED ? tiles_n : 1) > INT32_MAX) G2B_REFUSE("gemm_fp8_few: %d x %d is too large for one launch", p.M, p.N);
   p.tiles_n = (int)tiles_n;
   const dim3 grid((unsigned)(tiles_m * p.split * (GROUPED ? tiles_n : 1)), GROUPED ? 1u : (unsigned)tiles_n);
   g2b_launch_cluster(gemm_fp8_few_kernel<NX, LANES_A, EPI, GROUPED, FUSED>, grid, dim3(Shape<NX, LANES_A, FUSED, GROUPED>::THREADS),

@@ -56,15 +56,15 @@ static Choice choose(int M, int N, int blocks, int experts, bool rows_needed, Wa
   const long long each = ((long long)M + used - 1) / used;
   const double w_bytes = (double)used * N * blocks * F8_BLOCK;
   const double behind = rows_needed ? QUANTISED_FIRST + 1e-6 * M * N * 2.5 / 4 : 0;      // float, read and written again
-  const long long pairs_tiles = used * ((each + 255) / 256) * ((N + 255) / 256);
+  const long long pairs_tiles = used * ((each + 255) / 256) * (((long long)N + 255) / 256);
   const int pairs = many::resident();
   Choice best = {0, 1, 0};
   double least = way == ON_THE_WAY ? INFINITY : QUANTISED_FIRST + MANY_START + (double)((pairs_tiles + pairs - 1) / pairs) * (blocks * MANY_BLOCK + MANY_TILE);
   auto look = [&](int columns, bool x, const Cost &k, int (*resident)(int)) {
     if (way == (x ? GIVEN_ROWS : ON_THE_WAY)) return;
     const int rows_a = columns > 0 ? columns : 128, rows_w = columns > 0 ? 128 : 64;
-    const long long tiles = used * ((each + rows_a - 1) / rows_a) * ((N + rows_w - 1) / rows_w);
-    if (tiles > INT32_MAX / few::MOST_SPLIT) return;
+    const long long tiles_n = ((long long)N + rows_w - 1) / rows_w, tiles = used * ((each + rows_a - 1) / rows_a) * tiles_n;
+    if (tiles > INT32_MAX / few::MOST_SPLIT || (!experts && tiles_n > few::MOST_TILES_N)) return;
     for (int split = 1; split <= few::MOST_SPLIT && split <= blocks; ++split) {
       const double us = estimate(k, tiles, blocks, split, resident(split), w_bytes) + (x ? 0 : QUANTISED_FIRST) + behind;
       if (us < least) least = us, best = {columns, split, x};
