@@ -9,17 +9,31 @@ struct GluForm {
   float limit, offset, c1, c3;
 };
 
+// NaN where either is (fminf and fmaxf give the other one: the gate of a NaN would be -infinity, or a capped number).
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 __device__ __forceinline__ float glu_value(float gate, float up, const GluForm &f) {
-  const float g = fminf(gate, f.limit);
-  const float u = fminf(fmaxf(up, -f.limit), f.limit) + f.offset;
-  return g / (1.f + expf(-(g * fmaf(f.c3 * g, g, f.c1)))) * u;
+  const float g = min_or_nan(gate, f.limit);
+  const float u = min_or_nan(max_or_nan(up, -f.limit), f.limit) + f.offset;
+  const float slope = f.c3 == 0.f ? f.c1 : fmaf(f.c3 * g, g, f.c1);      // (zero times an infinite gate is no number)
+  return g / (1.f + expf(-(g * slope))) * u;
 }
 
 // The same from the fast exponential and division, for epilogues that round to bfloat16.
 __device__ __forceinline__ float glu_value_fast(float gate, float up, const GluForm &f) {
-  const float g = fminf(gate, f.limit);
-  const float u = fminf(fmaxf(up, -f.limit), f.limit) + f.offset;
-  return __fdividef(g, 1.f + __expf(-(g * fmaf(f.c3 * g, g, f.c1)))) * u;
+  const float g = min_or_nan(gate, f.limit);
+  const float u = min_or_nan(max_or_nan(up, -f.limit), f.limit) + f.offset;
+  const float slope = f.c3 == 0.f ? f.c1 : fmaf(f.c3 * g, g, f.c1);
+  return __fdividef(g, 1.f + __expf(-(g * slope))) * u;
 }
 
 // The plain form by itself: SiLU(gate) * up, a third of the operations.
