@@ -285,12 +285,20 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
       if (GATED) {
         const int n_out = p.N / 2, out0 = (n0 + col0) / 2;                        // 64 outputs a thread
         [[maybe_unused]] float most = 0.f;
+        // (what is left in float has 32 bits' precision; the fast forms, within 2^-20 or so, where four bits of it are kept)
+        constexpr bool FAST = EPI == EPI_GATED_ROWS;
         if (p.silu) {
 #pragma unroll
-          for (int j = 0; j < COLS / 2; ++j) sum[j] = silu_value_fast(sum[(j >> 3) * 16 + (j & 7)], sum[(j >> 3) * 16 + (j & 7) + 8]);
+          for (int j = 0; j < COLS / 2; ++j) {
+            const float g = sum[(j >> 3) * 16 + (j & 7)], u = sum[(j >> 3) * 16 + (j & 7) + 8];
+            sum[j] = FAST ? silu_value_fast(g, u) : silu_value(g, u);
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < COLS / 2; ++j) sum[j] = glu_value_fast(sum[(j >> 3) * 16 + (j & 7)], sum[(j >> 3) * 16 + (j & 7) + 8], p.form);
+          for (int j = 0; j < COLS / 2; ++j) {
+            const float g = sum[(j >> 3) * 16 + (j & 7)], u = sum[(j >> 3) * 16 + (j & 7) + 8];
+            sum[j] = FAST ? glu_value_fast(g, u, p.form) : glu_value(g, u, p.form);
+          }
         }
         if (out0 + COLS / 2 > n_out)                     // the last outputs' tile: zeros behind them
 #pragma unroll

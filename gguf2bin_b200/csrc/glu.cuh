@@ -37,6 +37,7 @@ __device__ __forceinline__ float glu_value_fast(float gate, float up, const GluF
 }
 
 // The plain form by itself: SiLU(gate) * up, a third of the operations.
+__device__ __forceinline__ float silu_value(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 __device__ __forceinline__ float silu_value_fast(float gate, float up) { return __fdividef(gate, 1.f + __expf(-gate)) * up; }
 
 // The activation alone: z * sigmoid(z (c1 + c3 z^2)).
