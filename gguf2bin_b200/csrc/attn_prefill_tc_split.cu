@@ -127,7 +127,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q,
                        const float *__restrict__ sink, int planes,
                        const bf16 *__restrict__ gate, int gate_stride, float cap_in2, float cap, int keep_first,
                        int v_heads) {
-  pdl_launch();
   // The swizzled panels need 1024-byte alignment.  The kernel has no static shared memory, so
   // the dynamic part starts at the aligned base of the window; checked rather than assumed.
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -166,7 +165,10 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q,
     mbar_init(o_ready, 2);                       // both issuers
     mbar_init_fence();
   }
-  if (warp == SOFTMAX_WARPS + 1) tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
+  if (warp == SOFTMAX_WARPS + 1) {
+    tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
+    pdl_launch();                               // only now: see tmem_alloc
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -111,7 +111,6 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   constexpr bool GATED = EPI == EPI_GATED_F32;
   constexpr int ADDERS = 4 * S::ADD, CHUNK = S::CHUNK, PIECE = S::COLS < 32 ? S::COLS : 32, PIECES = S::COLS / PIECE;
   constexpr uint32_t IDESC = (1u << 4) | ((uint32_t)(NX >> 3) << 17) | ((uint32_t)(LANES >> 4) << 24);      // accumulator float, operands e4m3, K-major
-  pdl_launch();
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float4 *sent = reinterpret_cast<float4 *>(smem);                        // [range][four columns owned][row], behind the loop
@@ -138,7 +137,11 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
   // Tensor memory under the wait for the kernel in front; but many tiles of experts, a part of them none, take theirs once they know (64 tokens of 6 choices:
   // 67.5 us against 70.4; one token, which quantises on the way: 17.2 against 16.0).
   constexpr bool EARLY = !GROUPED || FUSED;
-  if (EARLY && warp == ADDERS + 1) tmem_alloc(smem_addr(tmem_slot), S::TMEM);
+  auto take_tensor_memory = [&] {
+    tmem_alloc(smem_addr(tmem_slot), S::TMEM);
+    pdl_launch();                                        // only now: see tmem_alloc
+  };
+  if (EARLY && warp == ADDERS + 1) take_tensor_memory();
   tc_fence_before();
   int e = 0, m0 = tile_m * S::ROWS_A, end = p.M;
   if (GROUPED) {
@@ -209,7 +212,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
   }
   if (!EARLY) {
-    if (warp == ADDERS + 1) tmem_alloc(smem_addr(tmem_slot), S::TMEM);
+    if (warp == ADDERS + 1) take_tensor_memory();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

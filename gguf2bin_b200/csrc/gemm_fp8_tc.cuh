@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_out,
                    const __grid_constant__ Tc p) {
   constexpr bool GATED = EPI == EPI_GATED_F32 || EPI == EPI_GATED_ROWS;
-  pdl_launch();
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int OUT_BYTES = ADDERS * BOXES<GROUPED> * BOX_BYTES;
@@ -121,7 +120,10 @@ gemm_fp8_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     for (int b = 0; b < 2; ++b) mbar_init(sum_empty0 + 8 * b, 2 * ADDERS);      // in the first CTA: both CTAs' adders
     mbar_init_fence();
   }
-  if (warp == ADDERS + 1) tmem_alloc_pair(smem_addr(tmem_slot), 2 * BN);
+  if (warp == ADDERS + 1) {
+    tmem_alloc_pair(smem_addr(tmem_slot), 2 * BN);
+    pdl_launch();                                        // only now: see tmem_alloc
+  }
   pdl_wait();
   const int tiles_n = (p.N + BN - 1) / BN;
   int n_tiles;

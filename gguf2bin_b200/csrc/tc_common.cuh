@@ -123,7 +123,9 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 }
-// whole warp: allocate `cols` (power of two >= 32) tensor-memory columns, address to *slot
+// whole warp: allocate `cols` (power of two >= 32) tensor-memory columns, address to *slot.  It waits, without a bound, until the
+// multiprocessor has as many.  A kernel that was let in early holds its columns while it waits for the kernel in front, so that one has to have
+// its own: kernels that may share a multiprocessor with others whose columns and theirs are more than 512 call pdl_launch() behind this.
 __device__ __forceinline__ void tmem_alloc(uint32_t slot_smem, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot_smem), "r"(cols));
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
