@@ -29,7 +29,7 @@
 namespace few {
 
 constexpr int LANES = 128, BK = F8_BLOCK, LANE_BYTES = LANES * BK;
-enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36 };
+enum { ST_PRODUCER_TIMEOUT = 34, ST_MMA_TIMEOUT = 35, ST_ADDER_TIMEOUT = 36, ST_QUANTISER_TIMEOUT = 37 };
 
 constexpr int MOST_SPLIT = 8;
 constexpr int MOST_TILES_N = 65535;                      // a product's tiles along W's rows are the grid's second axis
@@ -322,7 +322,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
           ask(u, i + AHEAD);
           if (i >= S::STAGES) ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * s, (i / S::STAGES - 1) & 1));
           if (!ok) {
-            if (lane == 0) atomicExch(p.status, ST_PRODUCER_TIMEOUT);
+            if (lane == 0) atomicExch(p.status, ST_QUANTISER_TIMEOUT);
             break;
           }
           *reinterpret_cast<uint4 *>(smem + s * S::STAGE_BYTES + LANE_BYTES + r * 128 + ((part ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);

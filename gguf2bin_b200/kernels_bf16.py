@@ -117,7 +117,7 @@ def check_status() -> None:
                     11: "the TMA producer", 12: "the MMA issuer", 13: "a softmax warp",
                     21: "the TMA producer", 22: "the MMA issuer", 23: "an adder",
                     31: "the TMA producer", 32: "the MMA issuer", 33: "an adder",
-                    34: "the TMA producer", 35: "the MMA issuer", 36: "an adder"}.get(code, "a role")
+                    34: "the TMA producer", 35: "the MMA issuer", 36: "an adder", 37: "a quantising warp"}.get(code, "a role")
             raise KernelError(f"{kernel} on {dev}: {what} gave up waiting on a barrier (code {code}); "
                               "the result of that launch is invalid")
 
