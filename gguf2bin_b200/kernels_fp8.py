@@ -344,7 +344,7 @@ def moe_sort(idx: torch.Tensor, n_real: int, starts: torch.Tensor, pair_row: tor
     _call(f, _ptr(idx), idx.numel(), n_real, _ptr(starts), _ptr(pair_row), _ptr(row_pair), _stream())
 
 
-def _plan_experts(key, h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, pair_row, form) -> _Plan:
+def _plan_experts(key, h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, pair_row, form, forced) -> _Plan:
     what = "moe_experts_fp8"
     _check_matrix(what, w_gate_up, True, True)
     _check_matrix(what, w_down, False, True)
@@ -367,15 +367,22 @@ def _plan_experts(key, h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, 
     call.M, call.N, call.K, call.x_dtype, call.n_experts = h.shape[0], 2 * inter, w_gate_up.k, _code(h.dtype), n_experts
     call.top, call.H, call.x_stride, call.ldw = idx.shape[1], w_down.q.shape[1], h.stride(0), w_gate_up.q.shape[2]
     call.limit, call.offset, call.c1, call.c3 = form
-    return _plan(key, call, h.device, "g2b_fp8_experts_plan", "g2b_fp8_experts", [c_void_p] * 12, h.data_ptr() % 16 == 0)
+    if forced is not None:
+        (columns, call.split), (columns_2, call.split_2) = forced
+        call.columns, call.with_x = (16, 1) if columns == WITH_X else (columns, 0)
+        call.columns_2, call.with_x_2 = (16, 1) if columns_2 == WITH_X else (columns_2, 0)
+        if call.with_x != call.with_x_2:
+            raise KernelError(f"{what}: both products quantise their rows, or neither does")
+    return _plan(key, call, h.device, "g2b_fp8_experts_plan", "g2b_fp8_experts", [c_void_p] * 12, h.data_ptr() % 16 == 0, forced is None)
 
 
 def moe_experts(h: torch.Tensor, idx: torch.Tensor, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32: torch.Tensor, pair_row: torch.Tensor, form,
-                workspace) -> None:
+                workspace, forced=None) -> None:
+    """``forced``: the (columns, parts) of the gated and of the down products, as ``_product`` has them (None: what ``choose`` says)."""
     gq, gs, gk = w_gate_up
     dq, ds, dk = w_down
-    key = (_seen(h), _seen(idx), _seen(gq), _seen(gs), gk, _seen(dq), _seen(ds), dk, _seen(rows32), _seen(pair_row), form, _here())
-    plan = _plans.get(key) or _plan_experts(key, h, idx, w_gate_up, w_down, rows32, pair_row, form)
+    key = (_seen(h), _seen(idx), _seen(gq), _seen(gs), gk, _seen(dq), _seen(ds), dk, _seen(rows32), _seen(pair_row), form, _here(), forced)
+    plan = _plans.get(key) or _plan_experts(key, h, idx, w_gate_up, w_down, rows32, pair_row, form, forced)
     scratch, held = _scratch(plan, workspace, "fp8.experts", gq.device)
     n = plan.f(plan.at, h.data_ptr(), idx.data_ptr(), scratch, gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(), rows32.data_ptr(),
                pair_row.data_ptr(), plan.status, _stream())
