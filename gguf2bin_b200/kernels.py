@@ -23,7 +23,7 @@ __all__ = ["KernelError", "KernelBuildError", "embed_rows", "rmsnorm", "qknorm_r
            "proj_norm_rope_cache", "rotate_heads", "short_conv", "state_scan", "head_norm_gate", "gate_mul",
            "norm_add", "norm_shift", "scan_gates_step", "scan_gates_max", "state_readout", "pool_update", "moe_route", "moe_plan", "moe_gemm", "moe_gemv", "moe_gather", "moe_gemm_tc", "moe_combine", "moe_combine_norm_add", "moe_tile_rows", "tanh_norm", "scaled_join", "relu2", "selective_scan", "diff_combine", "GluForm", "norm_join", "moe_combine_join", "latent_pair",
            "channel_scan", "stream_add", "embed_norm_rows", "streams_read", "streams_join", "shift_mix", "latent_rope", "act_form", "linear_act", "linear_stacked", "head_expand_tiles",
-           "Fp8Rows", "Fp8Matrix", "Fp8Matrices", "quantize_rows", "quantize_matrix", "moe_sort", "moe_experts_fp8", "moe_back"]
+           "Fp8Rows", "Fp8Matrix", "Fp8Matrices", "quantize_rows", "quantize_matrix", "stored_matrix", "gate_up_matrix", "stack_matrices", "moe_sort", "moe_experts_fp8", "moe_back"]
 
 F32, BF16 = 0, 1
 EPI_STORE_F32, EPI_STORE_BF16, EPI_ACCUM_F32 = 0, 1, 2
@@ -784,6 +784,23 @@ def quantize_rows(x: torch.Tensor, rows: Fp8Rows, pair_row: Optional[torch.Tenso
 def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
     """A matrix [N, K], or a stack [E, N, K], of float32 or bfloat16 in 8 bits, a scale for every 128 x 128."""
     return (_fp8 or _fp8_mod()).quantize_matrix(w)
+
+
+def stored_matrix(q: torch.Tensor, scale: torch.Tensor) -> Fp8Matrix:
+    """A matrix from entries float8_e4m3fn [N, K] and the numbers float [ceil(N / 128), ceil(K / 128)] that its blocks are multiplied with, as a
+    checkpoint has them."""
+    return (_fp8 or _fp8_mod()).stored_matrix(q, scale)
+
+
+def gate_up_matrix(gate: Fp8Matrix, up: Fp8Matrix) -> Fp8Matrix:
+    """The matrix that ``gate_up_fused`` takes: the rows of two matrices of one size (a multiple of 8 of them) in eights in turn, each with its own
+    scales."""
+    return (_fp8 or _fp8_mod()).gate_up_matrix(gate, up)
+
+
+def stack_matrices(matrices) -> Fp8Matrix:
+    """Matrices of one size, gate/up ones or others, as the stack that ``moe_experts_fp8`` takes."""
+    return (_fp8 or _fp8_mod()).stack_matrices(matrices)
 
 
 def product_notices(what: str, w: Optional[torch.Tensor], compute_dtype: torch.dtype) -> list:

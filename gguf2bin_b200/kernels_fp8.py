@@ -186,10 +186,10 @@ def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
 
 def stored_matrix(q: torch.Tensor, scale: torch.Tensor) -> Fp8Matrix:
     """A checkpoint's matrix and the scales of its blocks; rows are filled up with zeros to whole blocks."""
-    n, k = q.shape
-    if q.dtype != F8 or tuple(scale.shape) != (blocks_of(n), blocks_of(k)):
-        raise KernelError(f"stored_matrix: float8_e4m3fn [{n}, {k}] goes with scales [{blocks_of(n)}, {blocks_of(k)}]; got {q.dtype} and "
-                          f"{list(scale.shape)}")
+    if q.dim() != 2 or q.dtype != F8 or tuple(scale.shape) != (blocks_of(q.shape[0]), blocks_of(q.shape[1])) or not scale.is_floating_point():
+        raise KernelError(f"stored_matrix: float8_e4m3fn [N, K] goes with a scale for every {BLOCK} x {BLOCK}; got {q.dtype} {list(q.shape)} and "
+                          f"{scale.dtype} {list(scale.shape)}")
+    k = q.shape[1]
     if k % BLOCK:
         q = torch.nn.functional.pad(q.view(torch.uint8), (0, blocks_of(k) * BLOCK - k)).view(F8)
     return Fp8Matrix(q.contiguous(), scale.to(torch.float32).contiguous(), k)
@@ -198,9 +198,9 @@ def stored_matrix(q: torch.Tensor, scale: torch.Tensor) -> Fp8Matrix:
 def gate_up_matrix(gate: Fp8Matrix, up: Fp8Matrix) -> Fp8Matrix:
     """Gate and up as one matrix, rows alternating in eights; the scales stay their own matrix's."""
     n = gate.q.shape[0]
-    if gate.k != up.k or up.q.shape[0] != n or n % 8:
-        raise KernelError(f"gate_up_matrix: two matrices of one size, rows a multiple of 8; got {list(gate.q.shape)} and {list(up.q.shape)}")
-    both = torch.stack([m.q.view(torch.uint8).view(n // 8, 8, -1) for m in (gate, up)], dim=1).reshape(2 * n, -1)
+    if gate.q.dim() != 2 or gate.scale.dim() != 2 or gate.k != up.k or up.q.shape != gate.q.shape or up.scale.shape != gate.scale.shape or n % 8:
+        raise KernelError(f"gate_up_matrix: two matrices of one size, rows a multiple of 8; got {list(gate.shape)} and {list(up.shape)}")
+    both = torch.stack([m.q.view(torch.uint8).reshape(n // 8, 8, -1) for m in (gate, up)], dim=1).reshape(2 * n, -1)
     return Fp8Matrix(both.view(F8), torch.stack([gate.scale, up.scale]).contiguous(), gate.k)
 
 
@@ -212,6 +212,10 @@ def no_matrix(n: int, k: int, device) -> Fp8Matrix:
 
 def stack_matrices(matrices) -> Fp8Matrix:
     """Matrices of one size as a stack (experts)."""
+    matrices = list(matrices)
+    if not matrices or any(m.q.dim() != 2 or m.k != matrices[0].k or m.q.shape != matrices[0].q.shape or m.scale.shape != matrices[0].scale.shape
+                           for m in matrices):
+        raise KernelError(f"stack_matrices: matrices of one size; got {[list(m.shape) for m in matrices[:4]]}")
     q = torch.stack([m.q.view(torch.uint8) for m in matrices])
     return Fp8Matrix(q.view(F8), torch.stack([m.scale for m in matrices]).contiguous(), matrices[0].k)
 
