@@ -10,6 +10,7 @@ they are.  Anything else in the object is refused, never ignored.
 from __future__ import annotations
 
 import dataclasses
+import re
 from typing import Any, Mapping
 
 from .specs import ConfigError, ModelSpec, PartSpec
@@ -45,6 +46,16 @@ def _module(name: str) -> str:
     return name[:-len(".weight")] if name.endswith(".weight") else name
 
 
+def _one_expert(left_out: str, module: str) -> bool:
+    """Whether ``left_out`` names ``module``, or what it is in, with a number in the place for an expert's."""
+    if "{}" not in module:
+        return False
+    pattern = re.escape(module).replace(re.escape("{}"), "[0-9]+").split(re.escape("."))
+    given = left_out.split(".")
+    numbered = next(i for i, p in enumerate(pattern) if "[0-9]+" in p)
+    return numbered < len(given) <= len(pattern) and all(re.fullmatch(p, g) for p, g in zip(pattern, given))
+
+
 def _converted(part: PartSpec, prefix: str, left_out: tuple) -> PartSpec:
     if part is None:
         return part
@@ -53,8 +64,11 @@ def _converted(part: PartSpec, prefix: str, left_out: tuple) -> PartSpec:
         params["shared"] = _converted(params["shared"], prefix, left_out)
     if part.kind in KINDS:
         names = dict(part["names"])
-        # (a name with a place for an expert's number stands for all of them: it is given here as it stands)
+        # (a name with a place for an expert's number stands for all of them)
         modules = [_module(prefix + names[k]) for k in KINDS[part.kind] if k in names]
+        one = [n for n in left_out if any(_one_expert(n, m) for m in modules)]
+        if one:
+            raise ConfigError(f"config.json: modules_to_not_convert leaves out {', '.join(one)} but not all matrices of that {part.kind}")
         out = [m for m in modules if any(m == n or m.startswith(n + ".") for n in left_out)]
         if out and len(out) < len(modules):
             raise ConfigError(f"config.json: modules_to_not_convert leaves out {', '.join(out)} but not all matrices of that {part.kind}")
