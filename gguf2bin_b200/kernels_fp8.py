@@ -13,7 +13,8 @@ from .kernels import SILU, Fp8Matrices, Fp8Matrix, Fp8Rows, KernelError, _call, 
 ON_THE_WAY = 16                      # rows up to which a product quantises them itself (csrc/products_fp8.cu, choose)
 BLOCK = 128                          # values of a row, and of either side of a matrix, that share a scale
 F8 = torch.float8_e4m3fn
-MOST_EXPERTS = 1024                  # csrc/quant_fp8.cu
+MOST_EXPERTS = 1024                  # csrc/product_fp8.cuh
+SORTED_AT_ONCE = 32 * 32 * 8         # pairs that the sort's block walks on by (csrc/quant_fp8.cuh)
 EPI_BF16, EPI_F32, EPI_ADD_F32, EPI_GATED_F32, EPI_GATED_ROWS = 0, 1, 2, 3, 4
 
 
@@ -104,6 +105,12 @@ def _on_device(what: str, *tensors) -> None:
         raise KernelError(f"{what}: tensors on the devices {sorted(set(at))}, while the current device is {here}")
 
 
+def _check_counts(what: str, *counts) -> None:
+    """Rows, columns and pairs are 32-bit numbers in the launchers."""
+    if max(counts) >= 2 ** 31:
+        raise KernelError(f"{what}: {max(counts)} are too many for one call")
+
+
 def _check_rows(what: str, rows: Fp8Rows, k: int, written: bool = False) -> None:
     q, s = rows
     kb = blocks_of(k)
@@ -154,6 +161,7 @@ def _plan_rows(key, x, rows: Fp8Rows, pair_row) -> tuple:
     tokens, k = x.shape
     if k < 1:
         raise KernelError("quantize_rows: rows without values")
+    _check_counts("quantize_rows", tokens, k, rows.q.shape[0])
     _check_rows("quantize_rows", rows, k, written=True)
     top = 1
     if pair_row is not None:
@@ -174,6 +182,7 @@ def quantize_matrix(w: torch.Tensor) -> Fp8Matrix:
     """A matrix [N, K], or a stack [E, N, K], in 8 bits with a scale for every 128 x 128."""
     if w.dim() not in (2, 3) or not w.is_contiguous() or 0 in w.shape:
         raise KernelError("quantize_matrix: a contiguous matrix, or a stack of them, that is not empty")
+    _check_counts("quantize_matrix", *w.shape)
     _on_device("quantize_matrix", w)
     n, k = w.shape[-2:]
     lead = tuple(w.shape[:-2])
@@ -249,6 +258,7 @@ def _plan_product(key, what: str, a, w: Fp8Matrix, out, epi: int, form, columns:
     as_rows, given = isinstance(out, Fp8Rows), isinstance(a, Fp8Rows)
     _check_matrix(what, w, gated, False)
     tokens = (a.q if given else a).shape[0]
+    _check_counts(what, tokens, w.q.shape[0], w.k)
     n = w.q.shape[0] // 2 if gated else w.q.shape[0]
     if as_rows:
         _check_rows(what, out, n, written=True)
@@ -343,6 +353,7 @@ def moe_sort(idx: torch.Tensor, n_real: int, starts: torch.Tensor, pair_row: tor
             continue
         if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() != n:
             raise KernelError(f"moe_sort: {what} is contiguous int32 of {n}; got {t.dtype} {list(t.shape)}")
+    _check_counts("moe_sort", idx.numel() + SORTED_AT_ONCE, n_real)
     _on_device("moe_sort", idx, starts, pair_row, row_pair)
     f = _f("g2b_moe_sort", [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
     _call(f, _ptr(idx), idx.numel(), n_real, _ptr(starts), _ptr(pair_row), _ptr(row_pair), _stream())
@@ -362,6 +373,7 @@ def _plan_experts(key, h, idx, w_gate_up: Fp8Matrix, w_down: Fp8Matrix, rows32, 
     if n_experts > MOST_EXPERTS:
         raise KernelError(f"{what}: {n_experts} experts, at most {MOST_EXPERTS}")
     n_pairs = idx.numel()
+    _check_counts(what, h.shape[0], n_pairs + SORTED_AT_ONCE, w_gate_up.q.shape[1], w_gate_up.k, w_down.q.shape[1])
     if rows32.dtype != torch.float32 or tuple(rows32.shape) != (n_pairs, w_down.q.shape[1]) or not rows32.is_contiguous():
         raise KernelError(f"{what}: the experts' rows are contiguous float32 [{n_pairs}, {w_down.q.shape[1]}]")
     if pair_row.dtype != torch.int32 or pair_row.numel() != n_pairs or not pair_row.is_contiguous():
@@ -409,6 +421,7 @@ def _plan_back(key, rows32, pair_row, weight, x_self, out, accumulate: bool) -> 
         raise KernelError("moe_back: weights [tokens, top] and an output [tokens, width]")
     tokens, top = weight.shape
     width = out.shape[1]
+    _check_counts("moe_back", tokens, top, width, rows32.shape[0])
     if weight.dtype != torch.float32 or not weight.is_contiguous() or pair_row.dtype != torch.int32 or not pair_row.is_contiguous() or \
             pair_row.numel() != tokens * top:
         raise KernelError(f"moe_back: weights are contiguous float32 [{tokens}, {top}], rows of the pairs as many int32")
