@@ -8,6 +8,7 @@
 #include "common.cuh"
 
 constexpr int F8_BLOCK = 128;
+constexpr int MOST_EXPERTS = 1024;                                     // of a routed layer: the sort has a thread for each, the products a list
 
 __device__ __forceinline__ float max_nan(float a, float b) {           // NaN where either is
   float r;

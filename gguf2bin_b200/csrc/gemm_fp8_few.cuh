@@ -17,12 +17,13 @@
 // ups of the same outputs, each with the scales of their own matrix.
 //
 // What bounds it: W's bytes where there are enough of them, else the way of a block of K: copy, four products and a commit (0.24 us of issue, whatever N
-// is and wherever W lies), tensor memory, sums.  Hence K in parts where tiles are few (each part more costs 0.6 us and its exchange), two CTAs a
+// is and wherever W lies), tensor memory, sums.  Hence K in parts where tiles are few (0.5 to 0.6 us, and 0.07 to 0.26 for each part), two CTAs a
 // multiprocessor, so that one's issue hides the other's, and 128 rows of A on the lanes from some 70 rows on (no factors from shared memory, 64 rows of W a
 // tile).  Measured, products behind one another in a graph, quantising included: 1 row by 6,144 x 4,096 6.8 us (25 MB), 8 rows' gate and up of 12,288 x 4,096
 // 18.4 (5.5 TB/s; a copy reaches 6.45), 64 by 5,120 x 17,408 18.2 with given rows (4.9 TB/s), 128 by 6,144 x 4,096 11.1, 256 by 4,096 x 4,096 10.9.
 //
-// Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
+// Every wait on a barrier gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu; the allocation of tensor memory waits for
+// CTAs that end whatever this one does (see tmem_alloc).
 #pragma once
 #include "product_fp8.cuh"
 
@@ -522,7 +523,7 @@ static cudaError_t allow() {
 }
 
 // How many CTAs in clusters of `split` the device holds at once.  The runtime counts one CTA a multiprocessor for a kernel that allocates tensor memory; there are
-// PER_SM (two: 148 tiles 4.6 us, 296 5.8, 444 9.6).
+// PER_SM, two or, of experts' rows in sixteens, three (two: 148 tiles 4.6 us, 296 5.8, 444 9.6).
 template <int NX, bool LANES_A, bool FUSED, bool GROUPED>
 static int resident(int split) {
   static G2bPerDevice kept[MOST_SPLIT + 1];

@@ -20,7 +20,8 @@
 // behind this one's last: 3 to 8 % slower).  The walk over all of it then meets the power cap: 2,048 rows by 6,144 x 4,096 50 us cool and 55 hot (2,060 and
 // 1,870 TFLOP/s), 8,192 by 4,096 x 12,288 added to a stream 382 and 441, gate and up of 17,408 x 5,120 at 2,048 rows 316 and 370 (2,310 and 1,970).
 //
-// Every wait gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu.
+// Every wait on a barrier gives up after a bounded number of polls and leaves a code in `*status`, as in gemm_tc.cu; the allocation of tensor memory waits for
+// CTAs that end whatever this one does (see tmem_alloc).
 #pragma once
 #include "product_fp8.cuh"
 

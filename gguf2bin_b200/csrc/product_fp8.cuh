@@ -9,7 +9,7 @@ using namespace tc;
 // stored in bfloat16, in float, added to float; the gate of two products in float, or as the quantised rows of the product behind it
 enum { EPI_BF16 = 0, EPI_F32 = 1, EPI_ADD_F32 = 2, EPI_GATED_F32 = 3, EPI_GATED_ROWS = 4 };
 
-constexpr int MOST_EXPERTS = 1024, MOST_INLINE = 32;
+constexpr int MOST_INLINE = 32;
 
 // C[t, n] = sum_b s[b, t] S[n / 128, b] sum_{k in block b} q[t, k] Q[n, k]:  a = q [M, lda] with sa = s [blocks, lds], or, in place of both, the
 // activations x themselves; w = Q [N, ldw] with sw = S [ceil(N / 128), blocks] (gated: gate and up rows in eights in turn, [2, ceil(N / 256), blocks]).

@@ -30,9 +30,12 @@ enum Way { EITHER_WAY, GIVEN_ROWS, ON_THE_WAY };
 // Microseconds that a product is estimated to take.  With `c` CTAs of `n` blocks of K each, as many as `most` at a time:
 //   start + (parts + part * split, where K is in parts) + the 4-norm of (the rounds of CTAs: n blocks each, and `wave` for every round but one) and
 //   (W's bytes at `rate` TB/s);  a block takes `alone` where no two CTAs share a multiprocessor, else `block`.
-// Fitted to 7,000 times of 430 products (1 to 1,500 rows, 256 to 30,000 outputs, K = 512 to 17,408; graphs of products behind one another): within
-// 7 to 10 % (root mean square of the logarithm); what the estimates choose is 2 % slower than the best choice in the mean, 26 at worst.  With the tiles the
-// largest that fit instead, 64 rows by 5,120 x 17,408 took 34 us (21), and 128 rows by 6,144 x 4,096 13.9 (11.1).
+// Fitted to 7,000 times of 430 products that are not experts' (1 to 1,500 rows, 256 to 30,000 outputs, K = 512 to 17,408; graphs of products behind one
+// another), within 7 to 10 % (root mean square of the logarithm); experts' are taken for as many rows each.  Against the best of all tiles and
+// parts that are looked at, with the kernels as they are: 150 products drawn from the same ranges lose 3.6 % in the mean and 25 at worst (73 rows by 14,912 x
+// 10,112 44.5 us, 35.6 with 128 rows on the lanes), 80 routed layers (1 to 2,048 tokens, 4 to 122 experts, popular ones among them) 1.0 % and 14.  Not looked at:
+// several tiles of rows quantised on the way, 29 rows by 960 x 512 5.4 us for 3.8.  With the tiles the largest that fit instead, 64 rows by 5,120 x 17,408
+// took 34 us (21), and 128 rows by 6,144 x 4,096 13.9 (11.1).
 struct Cost { double start, parts, part, alone, block, wave, rate; };
 constexpr Cost COST_X = {2.11, 0.60, 0.08, 0.348, 0.408, 1.82, 5.75}, COST_16 = {2.02, 0.59, 0.07, 0.238, 0.349, 1.77, 6.42},
                COST_32 = {2.57, 0.58, 0.08, 0.280, 0.411, 2.17, 6.46}, COST_64 = {2.81, 0.55, 0.18, 0.357, 0.550, 2.61, 5.27},

@@ -8,6 +8,9 @@
 //                    the choices alone.  starts[e] .. starts[e + 1]: the rows of expert e.  Pairs of experts from `n_real` on get no row (-1).
 //   moe_back         y_t = sum_j weight_tj (row of pair (t, j), or the token's own input where the pair has none), in the order of j.
 //
+// (moe.cu has both for experts of other types: moe_plan lists tiles for its products and gives places as its atomics fall, where here rows are quantised and
+// compared by place; moe_combine reads and stores float of any width, moe_back either type four values at a time.)
+//
 // All are bound by their bytes, or by their launch: 8,192 x 4,096 bfloat16 in 20.6 us (4.9 TB/s read and written), float 28 (6.0), 8,192 x 12,288 bfloat16 59;
 // 16,384 pairs sorted in 10.5 us, 4,096 rows of 2,048 to four places each 9.7, and back with weights 24.5 (5.6 TB/s).
 #pragma once
@@ -168,7 +171,8 @@ static int run_quantize_matrix(const void *w, int dtype, int count, int N, int K
 }
 
 // ---- pairs by expert --------------------------------------------------------------------------------------
-constexpr int SORT_WARPS = 32, SORT_MOST_EXPERTS = 1024, SORT_AHEAD = 8;
+constexpr int SORT_WARPS = 32, SORT_AHEAD = 8;
+static_assert(MOST_EXPERTS <= SORT_WARPS * 32, "an expert a thread");
 
 // One block.  A warp takes a stretch of the pairs, 32 at a time: lanes with one expert find each other (a ballot a bit of its number: match.any
 // takes 48 cycles of the multiprocessor: 27 us for 16,384 pairs, where this takes 12), the first of them counts for all.  No two warps share a counter, so
@@ -253,11 +257,11 @@ moe_sort_kernel(const int *__restrict__ idx, int n_pairs, int n_real, int bits, 
 
 // starts: int [n_real + 1]; row_pair (the pair of every row in use) may be null
 static int run_moe_sort(const int *idx, int n_pairs, int n_real, int *starts, int *pair_row, int *row_pair, cudaStream_t stream) {
-  if (n_real < 1 || n_real > SORT_MOST_EXPERTS) G2B_REFUSE("moe_sort: %d experts outside 1..%d", n_real, SORT_MOST_EXPERTS);
+  if (n_real < 1 || n_real > MOST_EXPERTS) G2B_REFUSE("moe_sort: %d experts outside 1..%d", n_real, MOST_EXPERTS);
   static G2bPerDevice configured;
   const int dev = g2b_current_device();
   if (dev < 0 || !configured.value[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * SORT_MOST_EXPERTS * 4);
+    const cudaError_t e = cudaFuncSetAttribute(moe_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SORT_WARPS * MOST_EXPERTS * 4);
     if (e != cudaSuccess) G2B_REFUSE("moe_sort: %s", cudaGetErrorString(e));
     if (dev >= 0) configured.value[dev] = 1;
   }

@@ -10,10 +10,10 @@ from . import kernels
 from .kernels_bf16 import _status, _status_word
 from .kernels import SILU, Fp8Matrices, Fp8Matrix, Fp8Rows, KernelError, _call, _code, _fn, _ptr, _stream
 
-ON_THE_WAY = 16                      # rows up to which a product quantises them itself (csrc/products_fp8.cu, choose)
+ON_THE_WAY = 16                      # rows up to which a product may quantise them itself (whether it does: choose in csrc/products_fp8.cu)
 BLOCK = 128                          # values of a row, and of either side of a matrix, that share a scale
 F8 = torch.float8_e4m3fn
-MOST_EXPERTS = 1024                  # csrc/product_fp8.cuh
+MOST_EXPERTS = 1024                  # csrc/fp8.cuh
 SORTED_AT_ONCE = 32 * 32 * 8         # pairs that the sort's block walks on by (csrc/quant_fp8.cuh)
 EPI_BF16, EPI_F32, EPI_ADD_F32, EPI_GATED_F32, EPI_GATED_ROWS = 0, 1, 2, 3, 4
 
