@@ -233,6 +233,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         for (int i = 0; i < ahead && !FUSED; ++i) tma_load_2d(smem_addr(smem + i * S::STAGE_BYTES) + at_a, &map_a, (kb0 + i) * BK, m0, full0 + 8 * i);
       }
       __syncwarp();
+      if (!GROUPED && FUSED) pdl_wait();
       for (int i = ahead; i < nkb; ++i) {
         const int s = i % S::STAGES;
         if (!__all_sync(0xffffffffu, mbar_wait(done0 + 8 * s, (i / S::STAGES - 1) & 1))) {
@@ -250,6 +251,7 @@ gemm_fp8_few_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
     }
     __syncwarp();
   } else if (warp == ADDERS + 1) {
+    if (!GROUPED) pdl_wait();                            // (the kernel in front may take longer than a wait is bounded by)
     for (int i = 0; i < nkb; ++i) {
       const int s = i % S::STAGES, h = i % S::NACC;
       const bool ok = mbar_wait(full0 + 8 * s, (i / S::STAGES) & 1) && (i < S::NACC || mbar_wait(sum_empty0 + 8 * h, (i / S::NACC - 1) & 1));

@@ -27,6 +27,8 @@ def all_units() -> list:
 # Builds that only the tests load: the tcgen05 kernels with a short wait limit and a copy role
 # that issues nothing, so that a test can see every other role give up and the kernel return.
 WAITS_RUN_OUT = ("G2B_SPIN_LIMIT=4096", "G2B_TEST_NO_PRODUCER")
+# Builds whose waits give up early, for a test that they begin where they should.
+SHORT_WAITS = ("G2B_SPIN_LIMIT=4096",)
 TEST_UNITS = [("gemm_tc.cu", WAITS_RUN_OUT), ("attn_prefill_tc.cu", ("HD=128",) + WAITS_RUN_OUT),
               ("attn_prefill_tc_split.cu", ("HD=128",) + WAITS_RUN_OUT), ("gemm_f32_tc.cu", WAITS_RUN_OUT),
-              ("products_fp8.cu", WAITS_RUN_OUT)]
+              ("products_fp8.cu", WAITS_RUN_OUT), ("products_fp8.cu", SHORT_WAITS)]
